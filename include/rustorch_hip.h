@@ -73,6 +73,7 @@ typedef struct rt_hip_ctx rt_hip_ctx;         /* executor: device, stream, scrat
 typedef struct rt_hip_qweight rt_hip_qweight; /* raw GGUF blocks resident in HBM */
 typedef struct rt_hip_llama rt_hip_llama;     /* weights + KV cache + decode-step state */
 typedef struct rt_hip_llama_batch rt_hip_llama_batch; /* KV caches and activations of several sequences decoded against one model */
+typedef struct rt_hip_paged_kv rt_hip_paged_kv; /* keys and values of many sequences in pages of one pool (one layer's) */
 typedef struct rt_hip_event rt_hip_event;     /* timing marker on the context's stream */
 
 typedef struct {
@@ -239,6 +240,62 @@ RT_HIP_API int rt_hip_attn_causal_dev(rt_hip_ctx *ctx, const float *q, const uin
 RT_HIP_API int rt_hip_add_dev(rt_hip_ctx *ctx, float *x, const float *y, size_t n);
 /* Greedy pick (SamplingConfig::greedy, example-cli/src/model/sampling.rs:28-35); ties -> lowest index. */
 RT_HIP_API int rt_hip_argmax_dev(rt_hip_ctx *ctx, const float *v, size_t n, int *out_index_dev);
+
+/* ---- a cache in pages: what KVCache::update (example-cli/src/model/transformer.rs:221-270) and the attention over it
+ *      (example-cli/src/model/architectures/attention.rs:233-338) become when many sequences share one pool of memory.
+ *      A pool holds n_pages pages of page_size positions (a power of two, 16..1024) of one layer:
+ *      [n_pages][n_kv_heads][page_size][head_dim] fp16, one array for the keys and one for the values (head_dim 64 or 128).
+ *      create allocates them (contents undefined), wrap_dev uses memory the caller keeps (16-byte aligned); pages returns
+ *      the two device pointers.
+ *      A batch is described by device arrays, read when the kernels run:
+ *        block_table [n_seq][max_blocks]  position p of sequence s is slot p % page_size of page block_table[s][p / page_size]
+ *        kv_len      [n_seq]              positions of sequence s, this call's new tokens included (0: nothing there yet)
+ *        cu_new      [n_seq + 1]          sequence s owns rows cu_new[s] .. cu_new[s + 1] - 1 of the new tokens, which are its
+ *                                         last positions; ascending
+ *      What they say is checked where it is used: a page id outside the pool is never followed (its positions are not stored
+ *      and not seen), a length beyond max_blocks * page_size counts as that, a row that no sequence owns is left as it was.
+ *      Sequences may share pages that are only read.  Rows of q, k, v and the outputs are *_ld floats apart (a multiple of 4, at
+ *      least the row's length), their bases 16-byte aligned; query head h reads key / value head h / (n_heads / n_kv_heads). */
+RT_HIP_API int rt_hip_paged_kv_create(rt_hip_ctx *ctx, size_t n_pages, int page_size, int n_kv_heads, int head_dim, rt_hip_paged_kv **out);
+RT_HIP_API int rt_hip_paged_kv_wrap_dev(rt_hip_ctx *ctx, uint16_t *k_pages, uint16_t *v_pages, size_t n_pages, int page_size, int n_kv_heads,
+                                        int head_dim, rt_hip_paged_kv **out);
+RT_HIP_API int rt_hip_paged_kv_free(rt_hip_ctx *ctx, rt_hip_paged_kv *kv);
+RT_HIP_API int rt_hip_paged_kv_pages(rt_hip_ctx *ctx, const rt_hip_paged_kv *kv, uint16_t **k_pages, uint16_t **v_pages);
+/* Store n_tok new tokens: keys turned by their positions and values go to the pages as fp16 (round to nearest even), queries
+ * (q may be NULL, then n_heads and q_out are ignored) are turned into q_out (which may be q itself, with the same distance
+ * between rows).  cu_new NULL: one token per sequence, n_tok = n_seq, and a sequence with kv_len 0 is idle (its rows are left
+ * alone).  rope: how the pairs of a head lie; pair i turns by position * theta^(-2i / head_dim), the angle taken in 64 bits. */
+typedef enum {
+    RT_HIP_ROPE_NONE = 0,        /* stored as given */
+    RT_HIP_ROPE_INTERLEAVED = 1, /* pairs (2i, 2i + 1), as rt_hip_rope_dev */
+    RT_HIP_ROPE_HALF = 2         /* pairs (i, i + head_dim / 2) */
+} rt_hip_rope;
+RT_HIP_API int rt_hip_paged_append_dev(rt_hip_ctx *ctx, const rt_hip_paged_kv *kv, const int *block_table, int max_blocks, const int *kv_len,
+                                       const int *cu_new, int n_seq, int n_tok, const float *k, size_t k_ld, const float *v, size_t v_ld,
+                                       const float *q, size_t q_ld, float *q_out, size_t q_out_ld, int n_heads, int rope, float theta);
+/* One query per sequence (row s of q) over its kv_len[s] positions: softmax(q.K^T / sqrt(head_dim)) . V per head; a sequence
+ * without positions gets zeros.  max_kv_len: the longest kv_len of the batch, which the launch is cut for (0 or too small
+ * costs time, never correctness).  Long sequences are split over workgroups and joined by a second launch; the partial
+ * results sit in the context's workspace. */
+RT_HIP_API int rt_hip_paged_attn_decode_dev(rt_hip_ctx *ctx, const rt_hip_paged_kv *kv, const int *block_table, int max_blocks, const int *kv_len,
+                                            int n_seq, int max_kv_len, const float *q, size_t q_ld, int n_heads, float *out, size_t out_ld);
+/* The new tokens of every sequence at once: row cu_new[s] + i (position kv_len[s] - (cu_new[s + 1] - cu_new[s]) + i) over the
+ * positions up to its own. */
+RT_HIP_API int rt_hip_paged_attn_prefill_dev(rt_hip_ctx *ctx, const rt_hip_paged_kv *kv, const int *block_table, int max_blocks, const int *kv_len,
+                                             const int *cu_new, int n_seq, int n_tok, const float *q, size_t q_ld, int n_heads, float *out,
+                                             size_t out_ld);
+
+/* ---- sampling on the device: SamplingConfig's temperature, top-k and top-p (example-cli/src/model/sampling.rs:8-80,118-274)
+ *      and min-p, one token per row of logits (rows ld floats apart) from given random numbers u in [0, 1).  The settings are
+ *      device arrays of one value per row; NULL, or a value that means nothing, switches a filter off: temperature <= 0 or
+ *      top_k 1 is the greedy pick (ties: lowest index; NULL temperature is 1), top_k <= 0, top_p outside (0, 1), min_p <= 0
+ *      are off.  The kept tokens: the top_k largest (equal logits: lower index first), of these the shortest prefix whose
+ *      probability reaches top_p of theirs, of these the ones at least min_p times as likely as the largest; the draw is the
+ *      first kept token by index whose running probability exceeds u.  NaN logits count as -inf; a row with nothing above -inf
+ *      reports -1.  out_prob (may be NULL): the probability the token was drawn with.  Probabilities are summed exactly
+ *      (64-bit integers); a token less likely than 2^-41 of the largest (2^-45 for 131072 tokens) is never drawn.  vocab up to 2^20. */
+RT_HIP_API int rt_hip_sample_dev(rt_hip_ctx *ctx, const float *logits, size_t ld, int n_rows, int vocab, const float *temperature, const int *top_k,
+                                 const float *top_p, const float *min_p, const double *u, int *out_token, float *out_prob);
 
 /* ---- the model object the CLI's InferenceEngine loop drives once per token
  *      (example-cli/src/model/inference.rs:91-211; GPTModel::forward, gpt.rs:192-263). */

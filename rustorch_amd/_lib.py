@@ -76,6 +76,18 @@ SIGNATURES = {
     "rt_hip_attn_causal_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p]),
     "rt_hip_add_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t]),
     "rt_hip_argmax_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]),
+    "rt_hip_paged_kv_create": (C.c_int, [C.c_void_p, C.c_size_t, C.c_int, C.c_int, C.c_int, c_void_pp]),
+    "rt_hip_paged_kv_wrap_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_int, C.c_int, c_void_pp]),
+    "rt_hip_paged_kv_free": (C.c_int, [C.c_void_p, C.c_void_p]),
+    "rt_hip_paged_kv_pages": (C.c_int, [C.c_void_p, C.c_void_p, c_void_pp, c_void_pp]),
+    "rt_hip_paged_append_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_size_t,
+                                          C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_void_p, C.c_size_t, C.c_int, C.c_int, C.c_float]),
+    "rt_hip_paged_attn_decode_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_size_t, C.c_int,
+                                               C.c_void_p, C.c_size_t]),
+    "rt_hip_paged_attn_prefill_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_void_p, C.c_size_t,
+                                                C.c_int, C.c_void_p, C.c_size_t]),
+    "rt_hip_sample_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_size_t, C.c_int, C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                    C.c_void_p, C.c_void_p]),
     "rt_hip_llama_create": (C.c_int, [C.c_void_p, C.POINTER(LlamaConfig), c_void_pp]),
     "rt_hip_llama_destroy": (C.c_int, [C.c_void_p, C.c_void_p]),
     "rt_hip_llama_upload_tensor": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_size_t, C.c_size_t, C.c_void_p, C.c_size_t]),

@@ -45,9 +45,18 @@ class DeviceBuffer:
     def __init__(self, ex: "HipKernelExecutor", nbytes: int):
         self.ex = ex
         self.nbytes = int(nbytes)
+        self.owns = True
         p = C.c_void_p()
         _lib.check(ex.lib.rt_hip_malloc(ex.ctx, self.nbytes, C.byref(p)), ex.ctx)
         self.ptr = p
+
+    @classmethod
+    def borrow(cls, ex: "HipKernelExecutor", ptr: int, nbytes: int) -> "DeviceBuffer":
+        """A buffer over device memory that someone else allocated and keeps (the memory of rt_hip_qweight_wrap_dev is another
+        such case).  The executor's stream is its own: work of another stream on that memory has to be waited for."""
+        buf = cls.__new__(cls)
+        buf.ex, buf.nbytes, buf.ptr, buf.owns = ex, int(nbytes), C.c_void_p(ptr), False
+        return buf
 
     @classmethod
     def from_host(cls, ex: "HipKernelExecutor", a: np.ndarray) -> "DeviceBuffer":
@@ -74,7 +83,8 @@ class DeviceBuffer:
 
     def free(self) -> None:
         if self.ptr:
-            self.ex.lib.rt_hip_free(self.ex.ctx, self.ptr)
+            if self.owns:
+                self.ex.lib.rt_hip_free(self.ex.ctx, self.ptr)
             self.ptr = C.c_void_p()
 
     def __del__(self):
@@ -104,6 +114,53 @@ class QWeight:
                 self.free()
         except Exception:
             pass
+
+
+class PagedKV:
+    """One layer's pool of pages (rt_hip_paged_kv): [n_pages][n_kv_heads][page_size][head_dim] fp16 keys and values."""
+
+    def __init__(self, ex: "HipKernelExecutor", handle: C.c_void_p, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, keep=()):
+        self.ex, self.handle, self._keep = ex, handle, keep
+        self.n_pages, self.page_size, self.n_kv_heads, self.head_dim = n_pages, page_size, n_kv_heads, head_dim
+        self.nbytes = 2 * n_pages * page_size * n_kv_heads * head_dim       # of the keys, and of the values
+
+    def pages(self) -> tuple[DeviceBuffer, DeviceBuffer]:
+        """The key pages and the value pages as buffers that this pool keeps."""
+        k, v = C.c_void_p(), C.c_void_p()
+        _lib.check(self.ex.lib.rt_hip_paged_kv_pages(self.ex.ctx, self.handle, C.byref(k), C.byref(v)), self.ex.ctx)
+        return DeviceBuffer.borrow(self.ex, k.value, self.nbytes), DeviceBuffer.borrow(self.ex, v.value, self.nbytes)
+
+    def free(self) -> None:
+        if self.handle:
+            self.ex.lib.rt_hip_paged_kv_free(self.ex.ctx, self.handle)
+            self.handle = C.c_void_p()
+
+    def __del__(self):
+        try:
+            if self.ex.ctx:
+                self.free()
+        except Exception:
+            pass
+
+
+class PagedSeqs:
+    """The device arrays that describe a batch of sequences over a pool: block_table [n_seq][max_blocks], kv_len [n_seq] and, for
+    ragged new tokens, cu_new [n_seq + 1] (all int32; their contents may change between calls); max_kv_len is the longest
+    kv_len, 0 when it is not known."""
+
+    def __init__(self, block_table: DeviceBuffer, kv_len: DeviceBuffer, n_seq: int, max_blocks: int, cu_new: DeviceBuffer | None = None, max_kv_len: int = 0):
+        if block_table.nbytes < 4 * n_seq * max_blocks or kv_len.nbytes < 4 * n_seq or (cu_new is not None and cu_new.nbytes < 4 * (n_seq + 1)):
+            raise ShapeMismatch("paged_seqs: arrays of %d, %d, %d bytes for n_seq=%d max_blocks=%d" % (
+                block_table.nbytes, kv_len.nbytes, cu_new.nbytes if cu_new is not None else 0, n_seq, max_blocks))
+        self.block_table, self.kv_len, self.n_seq, self.max_blocks, self.cu_new, self.max_kv_len = block_table, kv_len, n_seq, max_blocks, cu_new, max_kv_len
+
+
+def _rows(what: str, buf: DeviceBuffer, rows: int, row: int, ld: int | None) -> int:
+    """The distance between rows in floats, after checking that the buffer holds `rows` of them."""
+    ld = row if ld is None else ld
+    if rows and buf.nbytes < 4 * ((rows - 1) * ld + row):
+        raise ShapeMismatch("%s: a buffer of %d bytes for %d rows of %d floats, %d apart" % (what, buf.nbytes, rows, row, ld))
+    return ld
 
 
 class Event:
@@ -180,6 +237,10 @@ class HipKernelExecutor:
 
     def event(self) -> Event:
         return Event(self)
+
+    def borrow(self, ptr: int, nbytes: int) -> DeviceBuffer:
+        """A buffer over device memory allocated elsewhere; see DeviceBuffer.borrow."""
+        return DeviceBuffer.borrow(self, ptr, nbytes)
 
     def buffer(self, nbytes: int) -> DeviceBuffer:
         return DeviceBuffer(self, nbytes)
@@ -311,6 +372,78 @@ class HipKernelExecutor:
         buf = C.create_string_buffer(256)
         _lib.check(self.lib.rt_hip_qgemv_describe(self.ctx, n, wa, batch, buf, len(buf)), self.ctx)
         return buf.value.decode()
+
+    # -- a cache in pages (device buffers; every call enqueues only)
+    ROPE = {"none": 0, "interleaved": 1, "half": 2}
+
+    def paged_kv(self, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int) -> PagedKV:
+        """A pool of pages in memory of its own (contents undefined)."""
+        h = C.c_void_p()
+        _lib.check(self.lib.rt_hip_paged_kv_create(self.ctx, n_pages, page_size, n_kv_heads, head_dim, C.byref(h)), self.ctx)
+        return PagedKV(self, h, n_pages, page_size, n_kv_heads, head_dim)
+
+    def wrap_paged_kv(self, k_pages: DeviceBuffer, v_pages: DeviceBuffer, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int) -> PagedKV:
+        """A pool over two buffers that the caller keeps."""
+        need = 2 * n_pages * page_size * n_kv_heads * head_dim
+        if k_pages.nbytes < need or v_pages.nbytes < need:
+            raise ShapeMismatch("wrap_paged_kv: buffers of %d and %d bytes for pages of %d" % (k_pages.nbytes, v_pages.nbytes, need))
+        h = C.c_void_p()
+        _lib.check(self.lib.rt_hip_paged_kv_wrap_dev(self.ctx, k_pages.ptr, v_pages.ptr, n_pages, page_size, n_kv_heads, head_dim, C.byref(h)), self.ctx)
+        return PagedKV(self, h, n_pages, page_size, n_kv_heads, head_dim, keep=(k_pages, v_pages))
+
+    def paged_seqs(self, block_table: DeviceBuffer, kv_len: DeviceBuffer, n_seq: int, max_blocks: int, cu_new: DeviceBuffer | None = None,
+                   max_kv_len: int = 0) -> PagedSeqs:
+        return PagedSeqs(block_table, kv_len, n_seq, max_blocks, cu_new, max_kv_len)
+
+    def paged_append_dev(self, kv: PagedKV, seqs: PagedSeqs, k: DeviceBuffer, v: DeviceBuffer, n_tok: int, q: DeviceBuffer | None = None,
+                         q_out: DeviceBuffer | None = None, n_heads: int = 0, rope: str = "interleaved", theta: float = 10000.0, k_ld: int | None = None,
+                         v_ld: int | None = None, q_ld: int | None = None, q_out_ld: int | None = None) -> None:
+        """Turn the new tokens' keys (and queries, into q_out) by their positions and store keys and values in the pages."""
+        if rope not in self.ROPE:
+            raise InvalidParameters("paged_append: rope is one of %s, got %r" % (", ".join(self.ROPE), rope))
+        if (q is None) != (q_out is None):
+            raise InvalidParameters("paged_append: q and q_out go together")
+        rowkv, row = kv.n_kv_heads * kv.head_dim, n_heads * kv.head_dim
+        k_ld, v_ld = _rows("paged_append: k", k, n_tok, rowkv, k_ld), _rows("paged_append: v", v, n_tok, rowkv, v_ld)
+        if q is not None:
+            q_ld, q_out_ld = _rows("paged_append: q", q, n_tok, row, q_ld), _rows("paged_append: q_out", q_out, n_tok, row, q_out_ld)
+        _lib.check(self.lib.rt_hip_paged_append_dev(self.ctx, kv.handle, seqs.block_table.ptr, seqs.max_blocks, seqs.kv_len.ptr,
+                                                    seqs.cu_new.ptr if seqs.cu_new is not None else None, seqs.n_seq, n_tok, k.ptr, k_ld, v.ptr, v_ld,
+                                                    q.ptr if q is not None else None, q_ld or 0, q_out.ptr if q_out is not None else None, q_out_ld or 0,
+                                                    n_heads, self.ROPE[rope], theta), self.ctx)
+
+    def paged_attn_decode_dev(self, kv: PagedKV, seqs: PagedSeqs, q: DeviceBuffer, n_heads: int, out: DeviceBuffer, q_ld: int | None = None,
+                              out_ld: int | None = None) -> None:
+        """out[s] = attention of the one query of sequence s over its kv_len[s] positions (zeros where there are none)."""
+        row = n_heads * kv.head_dim
+        q_ld, out_ld = _rows("paged_attn_decode: q", q, seqs.n_seq, row, q_ld), _rows("paged_attn_decode: out", out, seqs.n_seq, row, out_ld)
+        _lib.check(self.lib.rt_hip_paged_attn_decode_dev(self.ctx, kv.handle, seqs.block_table.ptr, seqs.max_blocks, seqs.kv_len.ptr, seqs.n_seq,
+                                                         seqs.max_kv_len, q.ptr, q_ld, n_heads, out.ptr, out_ld), self.ctx)
+
+    def paged_attn_prefill_dev(self, kv: PagedKV, seqs: PagedSeqs, q: DeviceBuffer, n_tok: int, n_heads: int, out: DeviceBuffer, q_ld: int | None = None,
+                               out_ld: int | None = None) -> None:
+        """The new tokens of every sequence (seqs.cu_new), each over the positions up to its own."""
+        if seqs.cu_new is None:
+            raise InvalidParameters("paged_attn_prefill: the batch has no cu_new")
+        row = n_heads * kv.head_dim
+        q_ld, out_ld = _rows("paged_attn_prefill: q", q, n_tok, row, q_ld), _rows("paged_attn_prefill: out", out, n_tok, row, out_ld)
+        _lib.check(self.lib.rt_hip_paged_attn_prefill_dev(self.ctx, kv.handle, seqs.block_table.ptr, seqs.max_blocks, seqs.kv_len.ptr, seqs.cu_new.ptr,
+                                                          seqs.n_seq, n_tok, q.ptr, q_ld, n_heads, out.ptr, out_ld), self.ctx)
+
+    # -- sampling (device buffers, enqueues only)
+    def sample_dev(self, logits: DeviceBuffer, n_rows: int, vocab: int, u: DeviceBuffer, out_token: DeviceBuffer, temperature: DeviceBuffer | None = None,
+                   top_k: DeviceBuffer | None = None, top_p: DeviceBuffer | None = None, min_p: DeviceBuffer | None = None,
+                   out_prob: DeviceBuffer | None = None, ld: int | None = None) -> None:
+        """One token per row of logits: sampling.py's temperature, top-k and top-p, and min-p, settings per row (f32; top_k and
+        out_token int32), from the random numbers u (f64, one per row)."""
+        ld = _rows("sample: logits", logits, n_rows, vocab, ld)
+        for name, buf, size in (("u", u, 8), ("out_token", out_token, 4), ("temperature", temperature, 4), ("top_k", top_k, 4), ("top_p", top_p, 4),
+                                ("min_p", min_p, 4), ("out_prob", out_prob, 4)):
+            if buf is not None and buf.nbytes < size * n_rows:
+                raise ShapeMismatch("sample: %s has %d bytes for %d rows" % (name, buf.nbytes, n_rows))
+        ptr = lambda b: b.ptr if b is not None else None  # noqa: E731
+        _lib.check(self.lib.rt_hip_sample_dev(self.ctx, logits.ptr, ld, n_rows, vocab, ptr(temperature), ptr(top_k), ptr(top_p), ptr(min_p), u.ptr,
+                                              out_token.ptr, ptr(out_prob)), self.ctx)
 
     # -- decode-step operators (host arrays in, host arrays out; each call goes through device buffers)
     def rmsnorm(self, x, gamma, eps: float) -> np.ndarray:

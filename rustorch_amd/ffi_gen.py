@@ -18,9 +18,9 @@ HEADER = ROOT / "include" / "rustorch_hip.h"
 DOC = ROOT / "INTEGRATION.md"
 BEGIN, END = "<!-- hip_ffi.rs: generated by python -m rustorch_amd.ffi_gen -->", "<!-- end of hip_ffi.rs -->"
 
-OPAQUE = {"rt_hip_ctx": "RtHipCtx", "rt_hip_qweight": "RtHipQWeight", "rt_hip_llama": "RtHipLlama", "rt_hip_llama_batch": "RtHipLlamaBatch", "rt_hip_event": "RtHipEvent"}
+OPAQUE = {"rt_hip_ctx": "RtHipCtx", "rt_hip_qweight": "RtHipQWeight", "rt_hip_llama": "RtHipLlama", "rt_hip_llama_batch": "RtHipLlamaBatch", "rt_hip_event": "RtHipEvent", "rt_hip_paged_kv": "RtHipPagedKv"}
 STRUCTS = {"rt_hip_devinfo": "RtHipDevInfo", "rt_hip_llama_config": "RtHipLlamaConfig"}
-SCALARS = {"int": "i32", "float": "f32", "size_t": "usize", "uint64_t": "u64", "uint16_t": "u16", "int8_t": "i8", "uint8_t": "u8",
+SCALARS = {"int": "i32", "float": "f32", "double": "f64", "size_t": "usize", "uint64_t": "u64", "uint16_t": "u16", "int8_t": "i8", "uint8_t": "u8",
            "char": "std::os::raw::c_char", "void": "std::ffi::c_void"}
 
 
@@ -114,7 +114,7 @@ def generate() -> str:
             lines.append("    pub %s: %s," % (nm, ty))
         lines.append("}")
     lines.append("")
-    for cname in ("rt_hip_status", "rt_ggml_type", "rt_hip_llama_slot"):
+    for cname in ("rt_hip_status", "rt_ggml_type", "rt_hip_rope", "rt_hip_llama_slot"):
         for k, v in enum_values(text, cname):
             lines.append("pub const %s: i32 = %d;" % (k, v))
         lines.append("")

@@ -178,6 +178,8 @@ using std::max;
 using std::min;
 inline void sincosf_emu(float a, float *s, float *c) { *s = std::sin(a); *c = std::cos(a); }
 #define sincosf sincosf_emu
+inline void sincospif(float a, float *s, float *c) { *s = (float)std::sin(3.14159265358979323846 * (double)a); *c = (float)std::cos(3.14159265358979323846 * (double)a); }
+inline int __popcll(unsigned long long v) { return __builtin_popcountll(v); }
 
 // ---- wave operations
 inline float __shfl_xor(float v, int mask, int = 64) {
@@ -185,6 +187,13 @@ inline float __shfl_xor(float v, int mask, int = 64) {
 }
 inline int __shfl_xor(int v, int mask, int = 64) { return (int)emu::wave_exchange((uint32_t)v, emu::lane_id() ^ mask); }
 
+inline unsigned long long __ballot(bool pred) {
+    const uint32_t mine = pred ? 1u : 0u;
+    const uint32_t *all = static_cast<const uint32_t *>(emu::wave_gather(&mine, sizeof mine));
+    unsigned long long r = 0;
+    for (int l = 0; l < 64; l++) r |= (unsigned long long)(all[l] & 1u) << l;
+    return r;
+}
 inline int emu_update_dpp(int old, int src, int ctrl, int row_mask, int /*bank_mask*/, bool /*bound_ctrl*/) {
     int l = emu::lane_id(), from = l;
     bool write = ((row_mask >> (l >> 4)) & 1) != 0;
