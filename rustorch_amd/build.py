@@ -22,7 +22,7 @@ OBJ = PKG / "build"
 LIB_SO = PKG / "librustorch_hip.so"
 LIB_A = PKG / "librustorch_hip.a"
 
-SOURCES = ["rt_api.hip", "rt_kernels.hip", "rt_attn_prefill.hip", "rt_gemv.hip", "rt_gemv_mb.hip", "rt_gemm.hip", "rt_hgemm.hip", "rt_paged.hip", "rt_sample.hip", "rt_llama.hip", "rt_synth.cpp"]
+SOURCES = ["rt_api.hip", "rt_kernels.hip", "rt_attn_prefill.hip", "rt_gemv.hip", "rt_gemv_mb.hip", "rt_gemm.hip", "rt_hgemm.hip", "rt_paged.hip", "rt_paged_attn.hip", "rt_sample.hip", "rt_llama.hip", "rt_synth.cpp"]
 
 # -packed-fp32-ops off: v_pk_*_f32 forms are kept out of the generated code on purpose.
 HIP_FLAGS = [
@@ -50,7 +50,7 @@ def find_hipcc() -> str:
 # one of them a scratch frame (register spills or an array it could not keep in registers).  One spilling variant
 # inside such a kernel slows every launch of it, also the ones that never reach the variant.
 NO_SCRATCH = {"rt_gemv.hip": ("qgemv_kernel", "qgemv_lean_kernel"), "rt_gemm.hip": ("qgemm_kernel",), "rt_attn_prefill.hip": ("attn_causal_kernel",),
-              "rt_hgemm.hip": ("hgemm_kernel",), "rt_gemv_mb.hip": ("qgemv_mb_q4k_kernel", "qgemv_mb_q6k_kernel"),
+              "rt_hgemm.hip": ("hgemm_kernel",), "rt_gemv_mb.hip": ("qgemv_mb_q4k_kernel", "qgemv_mb_q6k_kernel"), "rt_paged_attn.hip": ("paged_decode_kernel",),
               "rt_kernels.hip": ("attn_decode_kernel", "attn_split_kernel", "attn_rows_kernel", "matmul_f32_mfma_kernel")}
 RESOURCE_FLAG = "-Rpass-analysis=kernel-resource-usage"
 

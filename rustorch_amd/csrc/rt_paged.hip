@@ -10,7 +10,7 @@
 // a length beyond the table's width counts as the width, and a row that no sequence owns is left as it was.
 // (The cache is the one KVCache::update of example-cli/src/model/transformer.rs:221-270 was meant to be, the attention the
 // masked scores / softmax / weighted sum of example-cli/src/model/architectures/attention.rs:233-338 over it.)
-#include "rt_device.h"
+#include "rt_paged.h"
 
 #include <new>
 
@@ -22,38 +22,6 @@ struct rt_hip_paged_kv {
 
 namespace rt {
 namespace {
-
-// What a launch knows of the pool and of the batch.
-struct PagedView {
-    uint16_t *k, *v;
-    const int *table, *kv_len, *cu_new;      // cu_new == nullptr: row s is the one new token of sequence s
-    int n_pages, page_shift, n_kv, n_seq, max_blocks;
-};
-
-// ------------------------------------------------------------------ which sequence and position a row belongs to
-// Whole waves call this (the sequences are looked at 64 at a time).  The row's sequence is the number of ends
-// cu_new[s + 1] <= t; false for a row that no sequence owns.
-__device__ __forceinline__ bool row_place(const PagedView &p, int t, int &seq, long long &pos) {
-    if (!p.cu_new) {
-        seq = t;
-        pos = (long long)p.kv_len[t] - 1;
-        return true;
-    }
-    const int lane = (int)(threadIdx.x & 63);
-    int before = 0;
-    for (int s0 = 0; s0 < p.n_seq; s0 += 64) {
-        const int s = s0 + lane;
-        const unsigned long long ended = __ballot(s < p.n_seq && p.cu_new[s + 1] <= t);
-        before += __popcll(ended);
-        if (ended != ~0ull) break;
-    }
-    if (before >= p.n_seq) return false;
-    const int a = p.cu_new[before], b = p.cu_new[before + 1];
-    if (t < a || t >= b) return false;
-    seq = before;
-    pos = (long long)p.kv_len[before] - b + t;
-    return true;
-}
 
 // --------------------------------------------------------------------------------------------------------- append
 // Element pair (a, b) of a head turns by pos * theta^(-2 i / head_dim): interleaved pairs (2i, 2i + 1) or halves
@@ -130,39 +98,6 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
             *reinterpret_cast<uint2 *>(dst + e1) = make_uint2((uint32_t)f2h_rne(y.x) | ((uint32_t)f2h_rne(y.y) << 16), (uint32_t)f2h_rne(y.z) | ((uint32_t)f2h_rne(y.w) << 16));
         }
     }
-}
-
-// ------------------------------------------------------------------------------------------------------- attention
-// One wave per (row, query head): the positions one after the other with a running maximum and sum.
-template <int HD>
-__global__ __launch_bounds__(64) void paged_attn_kernel(PagedView p, const float *q, size_t q_ld, int n_heads, float *out, size_t out_ld) {
-    constexpr int E = HD / 64;               // elements of the head a lane holds
-    const int h = blockIdx.x, t = blockIdx.y, lane = threadIdx.x;
-    int seq;
-    long long pos;
-    if (!row_place(p, t, seq, pos)) return;
-    const int kvh = h / (n_heads / p.n_kv);
-    const long long width = (long long)p.max_blocks << p.page_shift, n = min(pos + 1, width);
-    const float scale = 1.0f / sqrtf((float)HD);
-    float qv[E], acc[E], m = -INFINITY, l = 0.f;
-    for (int e = 0; e < E; e++) {
-        qv[e] = q[(size_t)t * q_ld + (size_t)h * HD + E * lane + e] * scale;
-        acc[e] = 0.f;
-    }
-    for (long long j = 0; j < n; j++) {
-        const int page = p.table[(size_t)seq * p.max_blocks + (size_t)(j >> p.page_shift)];
-        if (page < 0 || page >= p.n_pages) continue;
-        const size_t at = ((((size_t)page * p.n_kv + kvh) << p.page_shift) + (size_t)(j & ((1ll << p.page_shift) - 1))) * HD + E * lane;
-        float s = 0.f;
-        for (int e = 0; e < E; e++) s += qv[e] * h2f(p.k[at + e]);
-        s = wave_sum(s);
-        const float m_new = fmaxf(m, s);
-        const float keep = m_new == -INFINITY ? 1.f : expf(m - m_new), w = m_new == -INFINITY ? 0.f : expf(s - m_new);
-        l = l * keep + w;
-        for (int e = 0; e < E; e++) acc[e] = acc[e] * keep + w * h2f(p.v[at + e]);
-        m = m_new;
-    }
-    for (int e = 0; e < E; e++) out[(size_t)t * out_ld + (size_t)h * HD + E * lane + e] = l > 0.f ? acc[e] / l : (l == 0.f ? 0.f : l);
 }
 
 }  // namespace
@@ -320,14 +255,14 @@ int rt_hip_paged_attn_decode_dev(rt_hip_ctx *ctx, const rt_hip_paged_kv *kv, con
     RT_REQUIRE(ctx, q && out, RT_HIP_ERR_INVALID_ARG, "%s: NULL argument", who);
     RT_REQUIRE(ctx, max_kv_len >= 0, RT_HIP_ERR_INVALID_ARG, "%s: max_kv_len=%d", who, max_kv_len);
     if ((rc = heads_check(ctx, who, kv, n_heads))) return rc;
+    RT_REQUIRE(ctx, (long long)n_seq * n_heads <= 1 << 22, RT_HIP_ERR_SHAPE, "%s: %d sequences of %d heads are beyond one grid", who, n_seq, n_heads);
     const size_t row = (size_t)n_heads * kv->head_dim;
     if ((rc = rows_check(ctx, who, "q", q, q_ld, row)) || (rc = rows_check(ctx, who, "out", out, out_ld, row))) return rc;
     Guard g(ctx);
     const rt::PagedView p = view_of(kv, block_table, max_blocks, kv_len, nullptr, n_seq);
-    const dim3 grid((unsigned)n_heads, (unsigned)n_seq);
-    if (kv->head_dim == 128) rt::paged_attn_kernel<128><<<grid, 64, 0, ctx->stream>>>(p, q, q_ld, n_heads, out, out_ld);
-    else rt::paged_attn_kernel<64><<<grid, 64, 0, ctx->stream>>>(p, q, q_ld, n_heads, out, out_ld);
-    RT_TRY_HIP(ctx, hipGetLastError());
+    rc = rt::ensure_scratch(ctx, rt::paged_decode_bytes(p, kv->head_dim, n_heads, max_kv_len));
+    if (rc) return rc;
+    RT_TRY_HIP(ctx, rt::launch_paged_decode(ctx->stream, p, kv->head_dim, max_kv_len, q, q_ld, n_heads, out, out_ld, ctx->scratch));
     return RT_HIP_OK;
 }
 
@@ -345,10 +280,7 @@ int rt_hip_paged_attn_prefill_dev(rt_hip_ctx *ctx, const rt_hip_paged_kv *kv, co
     if (n_tok == 0) return RT_HIP_OK;
     Guard g(ctx);
     const rt::PagedView p = view_of(kv, block_table, max_blocks, kv_len, cu_new, n_seq);
-    const dim3 grid((unsigned)n_heads, (unsigned)n_tok);
-    if (kv->head_dim == 128) rt::paged_attn_kernel<128><<<grid, 64, 0, ctx->stream>>>(p, q, q_ld, n_heads, out, out_ld);
-    else rt::paged_attn_kernel<64><<<grid, 64, 0, ctx->stream>>>(p, q, q_ld, n_heads, out, out_ld);
-    RT_TRY_HIP(ctx, hipGetLastError());
+    RT_TRY_HIP(ctx, rt::launch_paged_prefill(ctx->stream, p, kv->head_dim, n_tok, q, q_ld, n_heads, out, out_ld));
     return RT_HIP_OK;
 }
 

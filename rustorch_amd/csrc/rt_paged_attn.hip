@@ -1,0 +1,430 @@
+// Attention of new queries over keys and values in pages (rt_paged.hip says how they lie):
+//   scores_j = (q . k_j) / sqrt(head_dim);  p = softmax(scores) with max subtraction;  out = sum_j p_j v_j
+// (example-cli/src/model/architectures/attention.rs:233-338), f32 in and out, fp16 keys and values.
+#include "rt_paged.h"
+
+#include <algorithm>
+
+namespace rt {
+namespace {
+
+typedef _Float16 half8v __attribute__((ext_vector_type(8)));
+typedef float float4v __attribute__((ext_vector_type(4)));
+
+// ------------------------------------------------------------------------------------------- one query per sequence
+// Bound by reading keys and values once (2 * 2 * head_dim bytes per position and kv head), so everything else has to fit beside
+// the loads, for one query head per kv head as well as for sixteen.  Both products run on the matrix cores in shapes whose
+// operands are what a lane loads, with no exchange between lanes:
+//   S[key][head] = K . Q^T      v_mfma_f32_16x16x32_f16: lane (g = l / 16, c = l % 16) loads 16 bytes of key c; Q is split into
+//                               two halves (value = hi + lo, after a power-of-two scaling), f32 accuracy for two instructions;
+//                               the lane ends with the scores of head c and keys 4 g + r, r < 4
+//   O^T[dim][head] = V^T . P    v_mfma_f32_16x16x4_f32, k = g: the lane's register p_r is the second operand as it stands if the
+//                               first is the value row 4 g + r, of which the lane loads chunk c: element e of the chunk is
+//                               dim VE c + e, so there is one accumulator per e
+// A lane's maximum and sum therefore belong to the head whose probabilities and outputs it holds.  The f32 products take a
+// third of the matrix cores' time at the rate the loads arrive at.
+// A workgroup of four waves takes one chunk of one sequence's positions for up to 16 query heads of one kv head; its waves take
+// tiles of 16 G positions in turn and meet at the end, through LDS.  The next tile's keys and values are requested before the
+// current one is used.
+// Chunks are equally long whatever the sequences are, so that a batch of one long and many short ones keeps every compute unit
+// busy to the end: the chunk length comes from the sum of the lengths, and each workgroup finds its sequence by running sums of
+// the chunk counts (64 sequences at a time, one load and a few lane exchanges).  A sequence of one chunk is finished at once;
+// the chunks of a longer one are joined by paged_join_kernel.
+// Measured (keys and values of three batches in turn, so that none stay in the last-level cache): 537 MB of one sequence of 131071
+// positions 95.5 us (5.6 TB/s), 837 MB of 48 sequences 163 us (5.1 TB/s), 278 MB of 33 sequences 63 us (4.4 TB/s), join included;
+// the join alone takes 4 to 5 us.  A copy of 4 GiB moves 4.6 TB/s.
+constexpr int kDecodeWaves = 4, kChunkUnit = 128, kHeadsPerBlock = 16, kChunkMinUnits = 2;
+
+__device__ __forceinline__ int length_of(const PagedView &p, int seq) {      // the table's width is at most 2^30 positions
+    return seq < p.n_seq ? max(0, min(p.kv_len[seq], p.max_blocks << p.page_shift)) : 0;
+}
+
+struct DecodeArgs {
+    PagedView p;
+    const float *q;
+    float *out;
+    size_t q_ld, out_ld;
+    int n_heads, group, head_blocks;
+    int budget;              // chunks that all sequences together may have beyond one each; 0: every sequence is one chunk
+    float *part;             // [chunk][n_heads][HD] of the sequences with several chunks, and behind it {max, sum} per entry
+    float2 *part_ml;
+    int2 *plan;              // [n_seq]: first chunk and number of chunks of each sequence, for the join
+};
+
+__device__ __forceinline__ int units_of(int len) { return (len + kChunkUnit - 1) / kChunkUnit; }
+// Units per chunk: whole waves call this, every wave of the grid gets the same answer.  sum(units) / budget, rounded up past
+// the sum's own rounding, so that sum over sequences of ceil(units / chunk) <= budget + n_seq.
+__device__ __forceinline__ int chunk_units(const PagedView &p, int budget) {
+    if (budget == 0) return 1 << 30;
+    float total = 0.f;
+    for (int s0 = 0; s0 < p.n_seq; s0 += 64) total += (float)units_of(length_of(p, s0 + (int)(threadIdx.x & 63)));
+    total = wave_sum(total);
+    return max(kChunkMinUnits, (int)fminf(total * 1.0002f / (float)budget, 1e9f) + 1);
+}
+__device__ __forceinline__ int chunks_of(int units, int per_chunk) { return max(1, (units + per_chunk - 1) / per_chunk); }
+
+template <int HD, int G, int OCC>
+__global__ __launch_bounds__(64 * kDecodeWaves, OCC) void paged_decode_kernel(DecodeArgs a) {
+    constexpr int KK = HD / 32, VE = HD / 16, kTileKeys = 16 * G;
+    typedef _Float16 halfv __attribute__((ext_vector_type(VE)));
+    constexpr int PS = 4 * VE + 4;           // floats a lane leaves in LDS: its outputs, maximum, sum (16-byte rows)
+    __shared__ __align__(16) float part[kDecodeWaves * 64 * PS];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), c = lane & 15, g = lane >> 4;
+    const int heads = a.p.n_kv * a.head_blocks, unit = (int)(blockIdx.x / (unsigned)heads), hx = (int)(blockIdx.x % (unsigned)heads);
+    const int kvh = hx / a.head_blocks, hb = hx % a.head_blocks;
+    const PagedView &p = a.p;
+    const int head_in_group = hb * kHeadsPerBlock + c, head = kvh * a.group + head_in_group;
+    const bool has_head = head_in_group < a.group;
+
+    // ---- which chunk of which sequence
+    const int per_chunk = chunk_units(p, a.budget);
+    int seq = -1, nth = 0, chunks = 1, len = 0;
+    for (int s0 = 0, before = 0; s0 < p.n_seq; s0 += 64) {
+        const int its = length_of(p, s0 + lane), mine = s0 + lane < p.n_seq ? chunks_of(units_of(its), per_chunk) : 0;
+        int upto = mine;                     // running sum over the lanes
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int below = __shfl_up(upto, o);
+            if (lane >= o) upto += below;
+        }
+        const unsigned long long past = __ballot(before + upto > unit);
+        if (past) {
+            const int l = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
+            seq = s0 + l;
+            chunks = __builtin_amdgcn_readlane(mine, l);
+            len = __builtin_amdgcn_readlane(its, l);
+            nth = unit - before - (__builtin_amdgcn_readlane(upto, l) - chunks);
+            break;
+        }
+        before += __builtin_amdgcn_readlane(upto, 63);
+    }
+    if (seq < 0) return;                     // the grid is cut for the most chunks there may be
+    if (a.budget > 0 && nth == 0 && hx == 0 && threadIdx.x == 0) a.plan[seq] = make_int2(unit, chunks);
+    const int first = chunks == 1 ? 0 : nth * per_chunk * kChunkUnit;
+    const int n = chunks == 1 ? len : min(per_chunk * kChunkUnit, len - first);      // positions of this chunk (0: an empty sequence)
+    const int tiles = (n + kTileKeys - 1) / kTileKeys;
+
+    // ---- the queries: lane (g, c) holds dims 32 kk + 8 g .. + 7 of head c, split in two halves
+    half8v qhi[KK], qlo[KK];
+    float sscale;
+    {
+        float qf[KK][8], amax = 0.f;
+        const float *qp = a.q + (size_t)seq * a.q_ld + (size_t)(has_head ? head : kvh * a.group) * HD + 8 * g;
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) {
+            const float4 x = *reinterpret_cast<const float4 *>(qp + 32 * kk), y = *reinterpret_cast<const float4 *>(qp + 32 * kk + 4);
+            qf[kk][0] = x.x; qf[kk][1] = x.y; qf[kk][2] = x.z; qf[kk][3] = x.w;
+            qf[kk][4] = y.x; qf[kk][5] = y.y; qf[kk][6] = y.z; qf[kk][7] = y.w;
+#pragma unroll
+            for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(qf[kk][e]));
+        }
+        amax = fmaxf(amax, __shfl_xor(amax, 16));
+        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        int ex = 0;
+        if (amax > 0.f) frexpf(amax, &ex);               // amax = f * 2^ex, f in [0.5, 1)
+        ex = max(ex, -100);
+        const float qscale = ldexpf(1.0f, 14 - ex);
+        // scores in units of log2: exp2 is the hardware's own exponential
+        sscale = ldexpf(1.0f, ex - 14) * (1.44269504088896341f / sqrtf((float)HD));
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = qf[kk][e] * qscale;
+                const _Float16 hi = (_Float16)v;
+                qhi[kk][e] = hi;
+                qlo[kk][e] = (_Float16)(v - (float)hi);
+            }
+    }
+
+    // ---- the chunk's pages, 64 table entries at a time: one per lane, bad ids as -1
+    const int page0 = (int)(first >> p.page_shift);
+    int window = 0, entry = -1;                               // entry of lane l: table[page0 + 64 * window + l]
+    auto load_window = [&](int w) {
+        const int i = page0 + 64 * w + lane;
+        int id = i < p.max_blocks ? p.table[(size_t)seq * p.max_blocks + i] : -1;
+        entry = id >= 0 && id < p.n_pages ? id : -1;
+        window = w;
+    };
+    if (n > 0) load_window(0);
+
+    // ---- a tile: G groups of 16 consecutive positions, each inside one page
+    const size_t k_lane = (size_t)c * HD + 8 * g, v_lane = (size_t)(4 * g) * HD + VE * c;
+    const int in_page = (1 << p.page_shift) - 1, first_in_page = (int)(first & in_page);
+    half8v kreg[G][KK];
+    halfv vreg[G][4];
+    int ok = 0;                                          // bit i: group i lies on a page of the pool
+    auto request = [&](int t, half8v (&kr)[G][KK], halfv (&vr)[G][4], int &good) {
+        good = 0;
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+            const int at = first_in_page + t * kTileKeys + 16 * i, pg = at >> p.page_shift;     // positions behind the start of page0
+            if ((pg >> 6) != window) load_window(pg >> 6);
+            const int id = __builtin_amdgcn_readlane(entry, pg & 63);
+            good |= id >= 0 ? 1 << i : 0;
+            const size_t base = ((((size_t)max(id, 0) * p.n_kv + kvh) << p.page_shift) + (size_t)(at & in_page)) * HD;
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) kr[i][kk] = *reinterpret_cast<const half8v *>(p.k + base + k_lane + 32 * kk);
+#pragma unroll
+            for (int r = 0; r < 4; r++) vr[i][r] = *reinterpret_cast<const halfv *>(p.v + base + v_lane + (size_t)r * HD);
+        }
+    };
+    float4v acc[VE];
+#pragma unroll
+    for (int e = 0; e < VE; e++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) acc[e][r] = 0.f;
+    float m_run = -INFINITY, l_run = 0.f;
+
+    if (wave < tiles) request(wave, kreg, vreg, ok);
+    for (int t = wave; t < tiles; t += kDecodeWaves) {
+        half8v kn[G][KK];
+        halfv vn[G][4];
+        int okn = 0;
+        request(min(t + kDecodeWaves, tiles - 1), kn, vn, okn);      // past the end a tile is requested again: no branch around the loads
+
+        float4v s[G];
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+            s[i] = float4v{ 0.f, 0.f, 0.f, 0.f };
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) {
+                s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kreg[i][kk], qhi[kk], s[i], 0, 0, 0);
+                s[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kreg[i][kk], qlo[kk], s[i], 0, 0, 0);
+            }
+        }
+        const int left = n - t * kTileKeys;              // positions of the tile that are the chunk's
+        if (left >= kTileKeys && ok == (1 << G) - 1) {
+#pragma unroll
+            for (int i = 0; i < G; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) s[i][r] *= sscale;
+        } else {                                         // what is not seen scores -inf, and its values (stale, perhaps NaN) count as zeros
+#pragma unroll
+            for (int i = 0; i < G; i++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const bool seen = 16 * i + 4 * g + r < left && ((ok >> i) & 1);
+                    s[i][r] = seen ? s[i][r] * sscale : -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < VE; e++) vreg[i][r][e] = seen ? vreg[i][r][e] : (_Float16)0.f;
+                }
+        }
+        float mt = m_run;
+#pragma unroll
+        for (int i = 0; i < G; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) mt = fmaxf(mt, s[i][r]);
+        mt = fmaxf(mt, __shfl_xor(mt, 16));
+        mt = fmaxf(mt, __shfl_xor(mt, 32));
+        const float m_ref = mt == -INFINITY ? 0.f : mt;  // nothing seen yet
+        const float alpha = __builtin_amdgcn_exp2f(m_run - m_ref);
+        m_run = mt;
+        l_run *= alpha;
+#pragma unroll
+        for (int e = 0; e < VE; e++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) acc[e][r] *= alpha;
+#pragma unroll
+        for (int i = 0; i < G; i++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float w = __builtin_amdgcn_exp2f(s[i][r] - m_ref);
+                l_run += w;
+#pragma unroll
+                for (int e = 0; e < VE; e++) acc[e] = __builtin_amdgcn_mfma_f32_16x16x4f32((float)vreg[i][r][e], w, acc[e], 0, 0, 0);
+            }
+#pragma unroll
+        for (int i = 0; i < G; i++) {
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) kreg[i][kk] = kn[i][kk];
+#pragma unroll
+            for (int r = 0; r < 4; r++) vreg[i][r] = vn[i][r];
+        }
+        ok = okn;
+    }
+    l_run += __shfl_xor(l_run, 16);
+    l_run += __shfl_xor(l_run, 32);
+
+    // ---- the four waves' results meet in LDS; wave w finishes dims VE (4 g + w) .. of every head
+    float *mine = part + (wave * 64 + lane) * PS;
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int e = 0; e < VE; e += 4) *reinterpret_cast<float4 *>(mine + VE * r + e) = make_float4(acc[e][r], acc[e + 1][r], acc[e + 2][r], acc[e + 3][r]);
+    *reinterpret_cast<float2 *>(mine + 4 * VE) = make_float2(m_run, l_run);
+    __syncthreads();
+    float fw[kDecodeWaves], m_all = -INFINITY, l_all = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDecodeWaves; w++) {
+        fw[w] = part[(w * 64 + lane) * PS + 4 * VE];
+        m_all = fmaxf(m_all, fw[w]);
+    }
+    const float m_ref = m_all == -INFINITY ? 0.f : m_all;
+#pragma unroll
+    for (int w = 0; w < kDecodeWaves; w++) {
+        fw[w] = __builtin_amdgcn_exp2f(fw[w] - m_ref);           // a wave without positions reports -inf: factor 0
+        l_all += part[(w * 64 + lane) * PS + 4 * VE + 1] * fw[w];
+    }
+    if (!has_head) return;
+    float o[VE];
+#pragma unroll
+    for (int e = 0; e < VE; e++) o[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < kDecodeWaves; w++)
+#pragma unroll
+        for (int e = 0; e < VE; e += 4) {
+            const float4 x = *reinterpret_cast<const float4 *>(part + (w * 64 + lane) * PS + VE * wave + e);
+            o[e] += x.x * fw[w]; o[e + 1] += x.y * fw[w]; o[e + 2] += x.z * fw[w]; o[e + 3] += x.w * fw[w];
+        }
+    float *dst;
+    float inv = 1.f;
+    if (chunks == 1) {
+        dst = a.out + (size_t)seq * a.out_ld + (size_t)head * HD;
+        inv = l_all == 0.f ? 0.f : 1.0f / l_all;
+    } else {
+        const size_t slot = (size_t)unit * a.n_heads + head;
+        dst = a.part + slot * HD;
+        if (wave == 0 && g == 0) a.part_ml[slot] = make_float2(m_all, l_all);
+    }
+#pragma unroll
+    for (int e = 0; e < VE; e += 4)
+        *reinterpret_cast<float4 *>(dst + VE * (4 * g + wave) + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+}
+
+// The chunks of one (sequence, head): out = sum_j acc_j 2^(m_j - M) / sum_j l_j 2^(m_j - M).  HD / 4 threads read one chunk's
+// outputs; every such group runs over its chunks with a maximum of its own, and the groups meet in LDS: two dependent reads of
+// memory (the plan, the partial results) from start to end.
+constexpr int kJoinThreads = 256;
+template <int HD>
+__global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(DecodeArgs a) {
+    constexpr int TPR = HD / 4, ROWS = kJoinThreads / TPR;
+    __shared__ __align__(16) float4 sums[kJoinThreads];
+    __shared__ float2 rows[ROWS];
+    const int head = blockIdx.x, seq = blockIdx.y, tid = threadIdx.x, row = tid / TPR, d = tid % TPR;
+    const int2 plan = a.plan[seq];
+    if (plan.y == 1) return;                 // written by the kernel before
+    const float2 *ml = a.part_ml + (size_t)plan.x * a.n_heads + head;
+    const float *acc = a.part + ((size_t)plan.x * a.n_heads + head) * HD + 4 * d;
+    float m = -INFINITY, l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int j = row; j < plan.y; j += ROWS) {
+        const float2 x = ml[(size_t)j * a.n_heads];
+        const float4 v = *reinterpret_cast<const float4 *>(acc + (size_t)j * a.n_heads * HD);
+        const float m_new = fmaxf(m, x.x), m_ref = m_new == -INFINITY ? 0.f : m_new;
+        const float keep = __builtin_amdgcn_exp2f(m - m_ref), w = __builtin_amdgcn_exp2f(x.x - m_ref);
+        m = m_new;
+        l = l * keep + x.y * w;
+        o.x = o.x * keep + v.x * w; o.y = o.y * keep + v.y * w; o.z = o.z * keep + v.z * w; o.w = o.w * keep + v.w * w;
+    }
+    sums[tid] = o;
+    if (d == 0) rows[row] = make_float2(m, l);
+    __syncthreads();
+    if (tid >= TPR) return;
+    float m_all = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) m_all = fmaxf(m_all, rows[i].x);
+    const float m_ref = m_all == -INFINITY ? 0.f : m_all;
+    l = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < ROWS; i++) {
+        const float w = __builtin_amdgcn_exp2f(rows[i].x - m_ref);
+        const float4 v = sums[i * TPR + tid];
+        l += rows[i].y * w;
+        o.x += v.x * w; o.y += v.y * w; o.z += v.z * w; o.w += v.w * w;
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    *reinterpret_cast<float4 *>(a.out + (size_t)seq * a.out_ld + (size_t)head * HD + 4 * tid) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+}
+
+// Chunks beyond one per sequence that a launch may cut (0: none, and no join).
+//   * No position count above 256: every sequence is one chunk.  One chat of 200 positions, 32 heads: 8.5 us; cut in two and
+//     joined, 9.5 us.
+//   * Several sequences: about 1536 workgroups, two rounds of the three that a compute unit holds.  33 sequences of 1 to 4097
+//     positions, 8 kv heads: 71 us with 512 workgroups, 66 with 1024, 63 with 1536 and 2048; 48 sequences of 1000 to 16000, 4 kv
+//     heads: 188, 176, 163, 167.
+//   * One sequence: its chunks are equally long, one workgroup per compute unit ends level, and fewer streams read memory faster.
+//     131071 positions, 8 kv heads: 95.5 us with 256 workgroups, 101 with 512, 103 with 768, 109 with 1536.
+int decode_budget(const PagedView &p, int n_heads, int max_kv_len) {
+    const int group = n_heads / p.n_kv, head_blocks = (group + kHeadsPerBlock - 1) / kHeadsPerBlock;
+    const long long width = (long long)p.max_blocks << p.page_shift, longest = max_kv_len > 0 ? std::min((long long)max_kv_len, width) : width;
+    if (longest <= kChunkMinUnits * kChunkUnit) return 0;
+    const long long useful = (longest + kChunkMinUnits * kChunkUnit - 1) / (kChunkMinUnits * kChunkUnit) * p.n_seq;
+    return (int)std::max(1ll, std::min(useful, (p.n_seq == 1 ? 256ll : 1536ll) / (p.n_kv * head_blocks)));
+}
+
+}  // namespace
+
+size_t paged_decode_bytes(const PagedView &p, int head_dim, int n_heads, int max_kv_len) {
+    const size_t budget = (size_t)decode_budget(p, n_heads, max_kv_len);
+    return budget == 0 ? 0 : (budget + p.n_seq) * n_heads * ((size_t)head_dim + 2) * sizeof(float) + (size_t)p.n_seq * sizeof(int2);
+}
+
+hipError_t launch_paged_decode(hipStream_t s, const PagedView &p, int head_dim, int max_kv_len, const float *q, size_t q_ld, int n_heads, float *out,
+                               size_t out_ld, void *work) {
+    DecodeArgs a{ p, q, out, q_ld, out_ld, n_heads, n_heads / p.n_kv, 0, decode_budget(p, n_heads, max_kv_len), nullptr, nullptr, nullptr };
+    a.head_blocks = (a.group + kHeadsPerBlock - 1) / kHeadsPerBlock;
+    const size_t chunks = (size_t)a.budget + p.n_seq;
+    if (a.budget > 0) {
+        a.part = static_cast<float *>(work);
+        a.part_ml = reinterpret_cast<float2 *>(a.part + chunks * n_heads * head_dim);
+        a.plan = reinterpret_cast<int2 *>(a.part_ml + chunks * n_heads);
+    }
+    const dim3 grid((unsigned)(chunks * p.n_kv * a.head_blocks)), join((unsigned)n_heads, (unsigned)p.n_seq);
+    // 16 positions a tile and three workgroups per compute unit, against 32 and two: 163 for 164 us (48 sequences), 63 for 67 (33
+    // sequences); heads of 64, whose tiles are half as large: 32 positions
+    if (head_dim == 128) {
+        paged_decode_kernel<128, 1, 3><<<grid, 64 * kDecodeWaves, 0, s>>>(a);
+        if (a.budget > 0) paged_join_kernel<128><<<join, kJoinThreads, 0, s>>>(a);
+    } else {
+        paged_decode_kernel<64, 2, 4><<<grid, 64 * kDecodeWaves, 0, s>>>(a);
+        if (a.budget > 0) paged_join_kernel<64><<<join, kJoinThreads, 0, s>>>(a);
+    }
+    return hipGetLastError();
+}
+
+namespace {
+// One wave per (row, query head): the positions one after the other with a running maximum and sum.
+template <int HD>
+__global__ __launch_bounds__(64) void paged_attn_kernel(PagedView p, const float *q, size_t q_ld, int n_heads, float *out, size_t out_ld) {
+    constexpr int E = HD / 64;               // elements of the head a lane holds
+    const int h = blockIdx.x, t = blockIdx.y, lane = threadIdx.x;
+    int seq;
+    long long pos;
+    if (!row_place(p, t, seq, pos)) return;
+    const int kvh = h / (n_heads / p.n_kv);
+    const long long width = (long long)p.max_blocks << p.page_shift, n = min(pos + 1, width);
+    const float scale = 1.0f / sqrtf((float)HD);
+    float qv[E], acc[E], m = -INFINITY, l = 0.f;
+    for (int e = 0; e < E; e++) {
+        qv[e] = q[(size_t)t * q_ld + (size_t)h * HD + E * lane + e] * scale;
+        acc[e] = 0.f;
+    }
+    for (long long j = 0; j < n; j++) {
+        const int page = p.table[(size_t)seq * p.max_blocks + (size_t)(j >> p.page_shift)];
+        if (page < 0 || page >= p.n_pages) continue;
+        const size_t at = ((((size_t)page * p.n_kv + kvh) << p.page_shift) + (size_t)(j & ((1ll << p.page_shift) - 1))) * HD + E * lane;
+        float s = 0.f;
+        for (int e = 0; e < E; e++) s += qv[e] * h2f(p.k[at + e]);
+        s = wave_sum(s);
+        const float m_new = fmaxf(m, s);
+        const float keep = m_new == -INFINITY ? 1.f : expf(m - m_new), w = m_new == -INFINITY ? 0.f : expf(s - m_new);
+        l = l * keep + w;
+        for (int e = 0; e < E; e++) acc[e] = acc[e] * keep + w * h2f(p.v[at + e]);
+        m = m_new;
+    }
+    for (int e = 0; e < E; e++) out[(size_t)t * out_ld + (size_t)h * HD + E * lane + e] = l > 0.f ? acc[e] / l : (l == 0.f ? 0.f : l);
+}
+
+}  // namespace
+
+hipError_t launch_paged_prefill(hipStream_t s, const PagedView &p, int head_dim, int n_tok, const float *q, size_t q_ld, int n_heads, float *out, size_t out_ld) {
+    const dim3 grid((unsigned)n_heads, (unsigned)n_tok);
+    if (head_dim == 128) paged_attn_kernel<128><<<grid, 64, 0, s>>>(p, q, q_ld, n_heads, out, out_ld);
+    else paged_attn_kernel<64><<<grid, 64, 0, s>>>(p, q, q_ld, n_heads, out, out_ld);
+    return hipGetLastError();
+}
+
+}  // namespace rt

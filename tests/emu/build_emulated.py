@@ -21,7 +21,7 @@ ROOT = Path(__file__).resolve().parents[2]
 CSRC = ROOT / "rustorch_amd" / "csrc"
 EMU = ROOT / "tests" / "emu"
 CLANG = "/opt/rocm/llvm/bin/clang++"
-SOURCES = ["rt_api.hip", "rt_kernels.hip", "rt_gemv.hip", "rt_gemv_mb.hip", "rt_gemm.hip", "rt_hgemm.hip", "rt_attn_prefill.hip", "rt_paged.hip", "rt_sample.hip", "rt_llama.hip", "rt_synth.cpp"]
+SOURCES = ["rt_api.hip", "rt_kernels.hip", "rt_gemv.hip", "rt_gemv_mb.hip", "rt_gemm.hip", "rt_hgemm.hip", "rt_attn_prefill.hip", "rt_paged.hip", "rt_paged_attn.hip", "rt_sample.hip", "rt_llama.hip", "rt_synth.cpp"]
 
 
 def _match_back(src: str, end: int) -> int:

@@ -30,6 +30,8 @@
 #define __align__(n) __attribute__((aligned(n)))
 
 struct uint2 { uint32_t x, y; };
+struct int2 { int x, y; };
+inline int2 make_int2(int x, int y) { return int2{ x, y }; }
 struct alignas(16) uint4 { uint32_t x, y, z, w; };
 struct float2 { float x, y; };
 struct alignas(16) float4 { float x, y, z, w; };
@@ -187,6 +189,11 @@ inline float __shfl_xor(float v, int mask, int = 64) {
 }
 inline int __shfl_xor(int v, int mask, int = 64) { return (int)emu::wave_exchange((uint32_t)v, emu::lane_id() ^ mask); }
 
+inline int __shfl_up(int v, unsigned by, int = 64) {
+    const int l = emu::lane_id();
+    return (int)emu::wave_exchange((uint32_t)v, l >= (int)by ? l - (int)by : l);
+}
+inline int __ffsll(unsigned long long v) { return __builtin_ffsll((long long)v); }
 inline unsigned long long __ballot(bool pred) {
     const uint32_t mine = pred ? 1u : 0u;
     const uint32_t *all = static_cast<const uint32_t *>(emu::wave_gather(&mine, sizeof mine));
@@ -329,6 +336,38 @@ inline emu_f32x16 emu_mfma_f32_32x32x16_f16(emu_f16x8 a, emu_f16x8 b, emu_f32x16
     return c;
 }
 #define __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, cbsz, abid, blgp) emu_mfma_f32_32x32x16_f16(a, b, c)
+
+// v_mfma_f32_16x16x32_f16: lane l holds A[l % 16][8 (l / 16) .. +7] and B[8 (l / 16) .. +7][l % 16] as eight halves;
+// D register r of lane l is D[4 (l / 16) + r][l % 16].  v_mfma_f32_16x16x4_f32: the same with A[l % 16][l / 16], B[l / 16][l % 16].
+typedef float emu_f32x4 __attribute__((ext_vector_type(4)));
+inline emu_f32x4 emu_mfma_f32_16x16x32_f16(emu_f16x8 a, emu_f16x8 b, emu_f32x4 c) {
+    struct { emu_f16x8 a, b; } mine{ a, b };
+    const auto *all = static_cast<const decltype(mine) *>(emu::wave_gather(&mine, sizeof mine));
+    const int l = emu::lane_id(), col = l % 16;
+    for (int r = 0; r < 4; r++) {
+        const int row = 4 * (l / 16) + r;
+        double acc = c[r];
+        for (int kb = 0; kb < 4; kb++)
+            for (int j = 0; j < 8; j++) acc += (double)((float)all[16 * kb + row].a[j] * (float)all[16 * kb + col].b[j]);
+        c[r] = (float)acc;
+    }
+    return c;
+}
+#define __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, cbsz, abid, blgp) emu_mfma_f32_16x16x32_f16(a, b, c)
+inline emu_f32x4 emu_mfma_f32_16x16x4f32(float a, float b, emu_f32x4 c) {
+    struct { float a, b; } mine{ a, b };
+    const auto *all = static_cast<const decltype(mine) *>(emu::wave_gather(&mine, sizeof mine));
+    const int l = emu::lane_id(), col = l % 16;
+    for (int r = 0; r < 4; r++) {
+        const int row = 4 * (l / 16) + r;
+        float acc = c[r];
+        for (int kb = 0; kb < 4; kb++) acc = fmaf(all[16 * kb + row].a, all[16 * kb + col].b, acc);
+        c[r] = acc;
+    }
+    return c;
+}
+#define __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, cbsz, abid, blgp) emu_mfma_f32_16x16x4f32(a, b, c)
+#define __builtin_amdgcn_exp2f(x) std::exp2((float)(x))
 
 // v_mfma_f32_32x32x2f32: lane l holds A[l % 32][l / 32] and B[l / 32][l % 32]; D as for the other 32 x 32 shapes
 inline emu_f32x16 emu_mfma_f32_32x32x2f32(float a, float b, emu_f32x16 c) {
