@@ -9,7 +9,14 @@
 // Weights are 64-bit integers, round(w_i * 2^F) with 2^F * vocab <= 2^62: sums of them are exact in any order, so the cut and
 // the draw do not depend on how the row is split over threads, and a token is lost to rounding only below 2^-(F+1) of the
 // largest weight (F = 45 for a vocabulary of 131072).  32-bit sums would move the cuts of a large vocabulary by whole tokens.
+//
+// Three launches: sample_range_kernel finds each row's largest logit (and its smallest finite one), sample_histogram_kernel
+// counts and weighs the tokens by how far below it they are, both with a row split over as many workgroups as fill the device;
+// sample_finish_kernel, one workgroup per row, finds from the histogram the bins that the cuts fall into, ranks the tokens of
+// just those bins exactly, and draws.
 #include "rt_device.h"
+
+#include <algorithm>
 
 namespace rt {
 namespace {
@@ -60,43 +67,223 @@ __device__ __forceinline__ unsigned long long block_sum_u64(unsigned long long v
     return t;
 }
 
-constexpr int kSampleThreads = 1024;
+// ---- bins: a row's tokens by their distance d = M - l below the largest logit, up to the distance R beyond which the weight
+// rounds to zero (or the smallest finite logit, if that is nearer): the bin's number is floor(d * (kBins - 1) / R), which is
+// monotone in d.  The weight of a token is the weight of its bin's middle, from a table, times exp(-r), |r| <= 0.016, by its
+// series to the sixth power (the next term is below 2^-54): a dozen 64-bit operations where exp() takes four times as many.
+// The middle is the same rounded number in the table and in r, and so the product is as exact as exp() itself.
+constexpr int kBins = 1024, kFinishThreads = 1024, kListMost = 2048, kGroupSteps = 16;
 
-// One workgroup per row.  The cuts are found by bisection over the 32 bits of the logits' order, one pass over the row per bit.
-__global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
-    __shared__ unsigned long long red[kSampleThreads / 64];
-    __shared__ unsigned long long run[kSampleThreads];
-    __shared__ int tie[kSampleThreads];
-    __shared__ float redf[kSampleThreads / 64];
-    const int tid = threadIdx.x, r = blockIdx.x, V = a.vocab;
+struct RowRange { float top, low; int arg, pad; };        // of one split of a row: largest logit, smallest finite one, index of the largest
+struct SampleWork {
+    RowRange *range;                                       // [row][split]
+    unsigned long long *sum;                               // [row][kBins]
+    uint32_t *count;                                       // [row][kBins]
+    int row0, splits, per_split;                           // this launch's first row
+};
+
+struct RowBins {
+    double top, scale, width, inv_t;
+    float topf;
+};
+__device__ __forceinline__ RowBins row_bins(float top, float low, double T, int frac_bits) {
+    RowBins b;
+    const double reach = (double)(frac_bits + 1) * 0.69314718055994531 * T, span = (double)top - (double)low;
+    const double R = reach < span ? reach : span;
+    b.topf = top;
+    b.top = (double)top;
+    b.scale = R > 0.0 ? (double)(kBins - 1) / R : 0.0;
+    b.width = R / (double)(kBins - 1);
+    b.inv_t = 1.0 / T;
+    return b;
+}
+#pragma clang fp contract(off)
+__device__ __forceinline__ double bin_middle(const RowBins &b, int bin) { return ((double)bin + 0.5) * b.width; }
+__device__ __forceinline__ int bin_of(const RowBins &b, float x) {       // kBins: beyond the reach, NaN or infinite
+    const double at = (b.top - (double)x) * b.scale;
+    return at < (double)kBins ? (int)at : kBins;                         // false for NaN
+}
+__device__ __forceinline__ double table_entry(const RowBins &b, int bin, int frac_bits) { return ldexp(exp(-(bin_middle(b, bin) * b.inv_t)), frac_bits); }
+// the weight times 2^frac_bits
+__device__ __forceinline__ double binned_weight(const RowBins &b, float x, int bin, const double *table, int frac_bits) {
+    if (x == b.topf) return ldexp(1.0, frac_bits);
+    const double r = ((b.top - (double)x) - bin_middle(b, bin)) * -b.inv_t;
+    double e = fma(r, 1.0 / 720.0, 1.0 / 120.0);
+    e = fma(e, r, 1.0 / 24.0);
+    e = fma(e, r, 1.0 / 6.0);
+    e = fma(e, r, 0.5);
+    e = fma(e, r, 1.0);
+    e = fma(e, r, 1.0);
+    return table[bin] * e;
+}
+__device__ __forceinline__ unsigned long long whole(double w) {          // rounded to nearest, 0 <= w <= 2^51: the sum's last bits
+    return __builtin_bit_cast(unsigned long long, w + 4503599627370496.0) - 0x4330000000000000ull;
+}
+#pragma clang fp contract(fast)
+
+// What a row asks for.
+struct RowAsks {
+    double T, min_w;
+    float p;                      // 0: off
+    int k;                        // 0: off
+    bool greedy;
+};
+__device__ __forceinline__ RowAsks row_asks(const SampleArgs &a, int r) {
+    const float t = a.temperature ? a.temperature[r] : 1.0f, p = a.top_p ? a.top_p[r] : 0.f, low = a.min_p ? a.min_p[r] : 0.f;
+    RowAsks q;
+    q.k = a.top_k ? a.top_k[r] : 0;
+    q.greedy = !(t > 0.f) || q.k == 1;       // temperature 0: the largest, the lowest index among equals
+    if (q.k < 0 || q.k >= a.vocab) q.k = 0;
+    q.T = (double)t;
+    q.p = p > 0.f && p < 1.f ? p : 0.f;
+    q.min_w = low > 0.f ? fmin((double)low, 1.0) : 0.0;
+    return q;
+}
+
+// N values of a row, `step` apart from i on; NaN from `end` on.  The requests go out together.
+template <int N>
+__device__ __forceinline__ void load_steps(const float *x, int i, int step, int end, float (&v)[N]) {
+#pragma unroll
+    for (int j = 0; j < N; j++) v[j] = i + j * step < end ? x[i + j * step] : NAN;
+}
+
+// The range of one split of a row; also clears the split's share of the row's histogram.
+__global__ __launch_bounds__(256) void sample_range_kernel(SampleArgs a, SampleWork w) {
+    __shared__ float tops[4], lows[4];
+    __shared__ int args[4];
+    const int tid = threadIdx.x, split = blockIdx.x, row = blockIdx.y, r = w.row0 + row;
     const float *x = a.logits + (size_t)r * a.ld;
-
-    float top = -INFINITY;
-    for (int i = tid; i < V; i += kSampleThreads) top = fmaxf(top, x[i] != x[i] ? -INFINITY : x[i]);
-    top = block_max(top, redf);
-    const uint32_t top_order = logit_order(top);
-    if (top == -INFINITY) {                          // nothing to draw from
-        if (tid == 0) {
-            a.out_token[r] = -1;
-            if (a.out_prob) a.out_prob[r] = 0.f;
+    const int i0 = split * w.per_split, i1 = min(a.vocab, i0 + w.per_split);
+    float top = -INFINITY, low = INFINITY;
+    int arg = INT32_MAX;
+    for (int i = i0 + tid; i < i1; i += 8 * 256) {
+        float v[8];
+        load_steps(x, i, 256, i1, v);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            if (v[j] > top) { top = v[j]; arg = i + 256 * j; }          // NaN: false; ascending index: the lowest of equals
+            if (v[j] > -INFINITY && v[j] < low) low = v[j];
         }
-        return;
     }
-    const float tf = a.temperature ? a.temperature[r] : 1.0f, p_keep = a.top_p ? a.top_p[r] : 0.f, low = a.min_p ? a.min_p[r] : 0.f;
-    int k = a.top_k ? a.top_k[r] : 0;
-    if (!(tf > 0.f)) k = 1;                          // temperature 0: the largest, the lowest index among equals
-    if (k <= 0 || k > V) k = V;
-    const double T = k == 1 ? 1.0 : (double)tf, min_w = low > 0.f ? fmin((double)low, 1.0) : 0.0;
+    for (int o = 32; o > 0; o >>= 1) {
+        const float t2 = __shfl_xor(top, o), l2 = __shfl_xor(low, o);
+        const int a2 = __shfl_xor(arg, o);
+        if (t2 > top || (t2 == top && a2 < arg)) { top = t2; arg = a2; }
+        low = fminf(low, l2);
+    }
+    if ((tid & 63) == 0) { tops[tid >> 6] = top; lows[tid >> 6] = low; args[tid >> 6] = arg; }
+    __syncthreads();
+    if (tid == 0) {
+        for (int i = 1; i < 4; i++) {
+            if (tops[i] > top || (tops[i] == top && args[i] < arg)) { top = tops[i]; arg = args[i]; }
+            low = fminf(low, lows[i]);
+        }
+        w.range[(size_t)row * w.splits + split] = RowRange{ top, low, arg, 0 };
+    }
+    const int share = (kBins + w.splits - 1) / w.splits, b1 = min(kBins, (split + 1) * share);
+    for (int b = split * share + tid; b < b1; b += 256) {
+        w.sum[(size_t)row * kBins + b] = 0;
+        w.count[(size_t)row * kBins + b] = 0;
+    }
+}
+
+// The whole row's range; whole waves call this.
+__device__ __forceinline__ RowRange row_range(const SampleWork &w, int row) {
+    RowRange g{ -INFINITY, INFINITY, INT32_MAX, 0 };
+    for (int s = (int)(threadIdx.x & 63); s < w.splits; s += 64) {
+        const RowRange o = w.range[(size_t)row * w.splits + s];
+        if (o.top > g.top) { g.top = o.top; g.arg = o.arg; }
+        g.low = fminf(g.low, o.low);
+    }
+    for (int o = 32; o > 0; o >>= 1) {
+        const float t2 = __shfl_xor(g.top, o), l2 = __shfl_xor(g.low, o);
+        const int a2 = __shfl_xor(g.arg, o);
+        if (t2 > g.top || (t2 == g.top && a2 < g.arg)) { g.top = t2; g.arg = a2; }
+        g.low = fminf(g.low, l2);
+    }
+    return g;
+}
+
+__global__ __launch_bounds__(256) void sample_histogram_kernel(SampleArgs a, SampleWork w) {
+    __shared__ double table[kBins];
+    __shared__ unsigned long long sum[kBins];
+    __shared__ uint32_t count[kBins];
+    const int tid = threadIdx.x, split = blockIdx.x, row = blockIdx.y, r = w.row0 + row;
+    const float *x = a.logits + (size_t)r * a.ld;
+    const RowAsks q = row_asks(a, r);
+    const RowRange g = row_range(w, row);
+    if (q.greedy || g.top == -INFINITY || g.top == INFINITY) return;      // decided by the range alone, or without weights
+    const RowBins b = row_bins(g.top, g.low, q.T, a.frac_bits);
+    for (int i = tid; i < kBins; i += 256) {
+        table[i] = table_entry(b, i, a.frac_bits);
+        sum[i] = 0;
+        count[i] = 0;
+    }
+    __syncthreads();
+    const int i0 = split * w.per_split, i1 = min(a.vocab, i0 + w.per_split);
+    for (int i = i0 + tid; i < i1; i += 8 * 256) {
+        float v[8];
+        load_steps(x, i, 256, i1, v);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int bin = bin_of(b, v[j]);
+            if (bin < kBins) {
+                __hip_atomic_fetch_add(&sum[bin], whole(binned_weight(b, v[j], bin, table, a.frac_bits)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                __hip_atomic_fetch_add(&count[bin], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < kBins; i += 256)
+        if (count[i]) {
+            __hip_atomic_fetch_add(&w.sum[(size_t)row * kBins + i], sum[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            __hip_atomic_fetch_add(&w.count[(size_t)row * kBins + i], count[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+}
+
+// A token's place in the order: ascending keys are descending logits, ascending indexes among equals.
+__device__ __forceinline__ unsigned long long rank_key(float x, int i) { return ((unsigned long long)(uint32_t)~logit_order(x) << 32) | (uint32_t)i; }
+
+// Exclusive running sum over the workgroup's threads; red holds one value per wave, total the sum of all.
+__device__ __forceinline__ unsigned long long block_scan_u64(unsigned long long v, unsigned long long *red, unsigned long long &total) {
+    const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6);
+    unsigned long long s = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)s, o), hi = (uint32_t)__shfl_up((int)(uint32_t)(s >> 32), o);
+        if (lane >= o) s += ((unsigned long long)hi << 32) | lo;
+    }
+    __syncthreads();
+    if (lane == 63) red[wave] = s;
+    __syncthreads();
+    unsigned long long before = 0;
+    total = 0;
+    for (int i = 0; i < (int)(blockDim.x >> 6); i++) {
+        if (i == wave) before = total;
+        total += red[i];
+    }
+    return before + s - v;
+}
+
+// The row on its own, without bins: the cuts by bisection over the 32 bits of the logits' order, one pass over the row per bit.
+// For rows with infinite logits and for rows with more equal or nearly equal logits in one bin than the list of
+// sample_finish_kernel holds.  run: kFinishThreads entries, tie as many.
+__device__ void sample_by_bisection(const SampleArgs &a, int r, const RowAsks &q, float top, unsigned long long *run, int *tie, unsigned long long *red) {
+    const int tid = threadIdx.x, V = a.vocab, k = q.k > 0 ? q.k : V;
+    const float *x = a.logits + (size_t)r * a.ld;
+    const uint32_t top_order = logit_order(top);
+    const float p_keep = q.p;
+    const double T = q.T, min_w = q.min_w;
 
     // ---- the cut: tokens above `cut` stay, of those at `cut` the first `ties` by index
     auto count_from = [&](uint32_t o) {              // tokens at o or above
         unsigned long long n = 0;
-        for (int i = tid; i < V; i += kSampleThreads) n += logit_order(x[i]) >= o ? 1 : 0;
+        for (int i = tid; i < V; i += kFinishThreads) n += logit_order(x[i]) >= o ? 1 : 0;
         return block_sum_u64(n, red);
     };
     auto weight_from = [&](uint32_t o) {
         unsigned long long n = 0;
-        for (int i = tid; i < V; i += kSampleThreads)
+        for (int i = tid; i < V; i += kFinishThreads)
             if (logit_order(x[i]) >= o) n += fixed_weight(x[i], top, T, a.frac_bits);
         return block_sum_u64(n, red);
     };
@@ -141,7 +328,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     }
 
     // ---- the draw, by index: each thread owns consecutive tokens
-    const int per = (V + kSampleThreads - 1) / kSampleThreads, i0 = min(V, tid * per), i1 = min(V, i0 + per);
+    const int per = (V + kFinishThreads - 1) / kFinishThreads, i0 = min(V, tid * per), i1 = min(V, i0 + per);
     int mine = 0;
     for (int i = i0; i < i1; i++) mine += logit_order(x[i]) == cut ? 1 : 0;
     tie[tid] = mine;
@@ -160,7 +347,7 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     run[tid] = sum;
     __syncthreads();
     unsigned long long total = 0, before = 0;
-    for (int j = 0; j < kSampleThreads; j++) {
+    for (int j = 0; j < kFinishThreads; j++) {
         if (j == tid) before = total;
         total += run[j];
     }
@@ -183,11 +370,195 @@ __global__ __launch_bounds__(kSampleThreads) void sample_kernel(SampleArgs a) {
     }
 }
 
+__global__ __launch_bounds__(kFinishThreads) void sample_finish_kernel(SampleArgs a, SampleWork w) {
+    static_assert(kBins == kFinishThreads && kListMost % kFinishThreads == 0, "a thread owns a bin and so many places of the list");
+    constexpr int kMine = kListMost / kFinishThreads, kGroup = kGroupSteps * kFinishThreads;
+    __shared__ double table[kBins];
+    // keys and weights of the tokens in the bins that the cuts fall into
+    __shared__ unsigned long long list[kListMost], list_weight[kListMost];
+    __shared__ unsigned long long red[kFinishThreads / 64], shared64[6];
+    __shared__ int listed, shared32[4];
+    const int tid = threadIdx.x, row = blockIdx.x, r = w.row0 + row, V = a.vocab;
+    const float *x = a.logits + (size_t)r * a.ld;
+    const RowAsks q = row_asks(a, r);
+    const RowRange g = row_range(w, row);
+    if (g.top == -INFINITY || q.greedy) {                   // nothing to draw from, or nothing to draw
+        if (tid == 0) {
+            a.out_token[r] = g.top == -INFINITY ? -1 : g.arg;
+            if (a.out_prob) a.out_prob[r] = g.top == -INFINITY ? 0.f : 1.f;
+        }
+        return;
+    }
+    if (g.top == INFINITY) {
+        sample_by_bisection(a, r, q, g.top, list, reinterpret_cast<int *>(list_weight), red);
+        return;
+    }
+    const RowBins b = row_bins(g.top, g.low, q.T, a.frac_bits);
+    table[tid] = table_entry(b, tid, a.frac_bits);
+
+    // ---- the last key that stays
+    unsigned long long cut = ~0ull;
+    if (q.k > 0 || q.p > 0.f) {
+        const unsigned long long bin_sum = w.sum[(size_t)row * kBins + tid], bin_count = w.count[(size_t)row * kBins + tid];
+        unsigned long long n_all, s_all;
+        const unsigned long long n_before = block_scan_u64(bin_count, red, n_all), s_before = block_scan_u64(bin_sum, red, s_all);
+        const unsigned long long k = q.k > 0 && (unsigned long long)q.k < n_all ? (unsigned long long)q.k : 0;
+        if (tid == 0) {
+            listed = 0;
+            shared32[0] = kBins;                            // the bin that top-k ends in (kBins: none)
+            shared64[0] = shared64[1] = s_all;              // weight above that bin, weight with it
+            shared64[2] = shared64[3] = 0;                  // tokens above it, tokens in it
+            shared32[1] = 0;                                // first and last bin that top-p may end in
+            shared32[2] = -1;
+        }
+        __syncthreads();
+        if (k && n_before < k && k <= n_before + bin_count) {
+            shared32[0] = tid;
+            shared64[0] = s_before;
+            shared64[1] = s_before + bin_sum;
+            shared64[2] = n_before;
+            shared64[3] = bin_count;
+        }
+        __syncthreads();
+        const int k_bin = shared32[0];
+        const unsigned long long k_weight_above = shared64[0], k_above = shared64[2], k_in = shared64[3];
+        if (q.p > 0.f && bin_sum) {
+            // the weight of the top k lies between that of the bins above its last one and that with it
+            const double lo = (double)q.p * (double)k_weight_above, hi = (double)q.p * (double)shared64[1];
+            const double from = (double)s_before, to = (double)(s_before + bin_sum);
+            if (from < lo && lo <= to) shared32[1] = tid;
+            if (from < hi && hi <= to) shared32[2] = tid;
+        }
+        if (tid == 0) shared64[4] = 0;
+        __syncthreads();
+        const int p_first = shared32[1], p_last = shared32[2];
+        if (tid == p_first) shared64[5] = s_before;         // weight above the bins of top-p, read behind the next barrier
+        for (int i0 = tid; i0 < V; i0 += 8 * kFinishThreads) {
+            float v[8];
+            load_steps(x, i0, kFinishThreads, V, v);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int bin = bin_of(b, v[j]);
+                if (bin < kBins && (bin == k_bin || (bin >= p_first && bin <= p_last))) {
+                    const int at = __hip_atomic_fetch_add(&listed, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                    if (at < kListMost) {
+                        list[at] = rank_key(v[j], i0 + j * kFinishThreads);
+                        list_weight[at] = whole(binned_weight(b, v[j], bin, table, a.frac_bits));
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        const int n_list = listed;
+        if (n_list > kListMost) {
+            sample_by_bisection(a, r, q, g.top, list, reinterpret_cast<int *>(list_weight), red);
+            return;
+        }
+        // ---- every listed token's number and weight of listed tokens before it.  The listed bins are top-p's, one after the
+        // other, and top-k's, which is the last of them or comes behind them.
+        unsigned long long key[kMine], own[kMine], weight_before[kMine];
+        int rank[kMine];
+#pragma unroll
+        for (int m = 0; m < kMine; m++) {
+            const int i = tid + m * kFinishThreads;
+            key[m] = i < n_list ? list[i] : 0;
+            own[m] = i < n_list ? list_weight[i] : 0;
+            weight_before[m] = 0;
+            rank[m] = 0;
+        }
+        for (int j = 0; j < n_list; j++) {
+            const unsigned long long other = list[j], its = list_weight[j];
+#pragma unroll
+            for (int m = 0; m < kMine; m++)
+                if (other < key[m]) {
+                    rank[m]++;
+                    weight_before[m] += its;
+                }
+        }
+        const unsigned long long above_list = shared64[5];
+        double goal = (double)q.p * (double)s_all;
+        if (k) {
+            unsigned long long mine = 0;
+            const int k_from = n_list - (int)k_in;          // where the list's part in the bin of top-k begins
+#pragma unroll
+            for (int m = 0; m < kMine; m++)
+                if (tid + m * kFinishThreads < n_list && rank[m] >= k_from) {
+                    const unsigned long long nth = k_above + (unsigned long long)(rank[m] - k_from);
+                    if (nth < k) mine += own[m];
+                    if (nth == k - 1) shared64[4] = key[m];
+                }
+            mine = block_sum_u64(mine, red);                // its barriers publish shared64[4]
+            cut = shared64[4];
+            goal = (double)q.p * (double)(k_weight_above + mine);
+        }
+        if (q.p > 0.f) {
+            // the first token at which the weight reaches the goal; it is one of the listed, and not behind top-k's last
+#pragma unroll
+            for (int m = 0; m < kMine; m++)
+                if (tid + m * kFinishThreads < n_list && key[m] <= cut) {
+                    const unsigned long long before = above_list + weight_before[m];
+                    if ((double)before < goal && (double)(before + own[m]) >= goal) shared64[0] = key[m];
+                }
+            __syncthreads();
+            cut = shared64[0];
+        }
+    }
+    __syncthreads();                                        // the table; the list is free from here on
+
+    // ---- the draw, by index, over the tokens whose key is at most the cut: the group of kGroup tokens, then the step of the
+    // group, then the wave and the lane
+    const double min_w = ldexp(q.min_w, a.frac_bits);
+    auto weight_at = [&](float v, int i) -> double {        // 0: not kept; kept weights are whole()d by the caller
+        if (rank_key(v, i) > cut) return 0.0;
+        const int bin = bin_of(b, v);
+        if (bin >= kBins) return 0.0;
+        const double f = binned_weight(b, v, bin, table, a.frac_bits);
+        return f >= min_w ? f : 0.0;
+    };
+    unsigned long long total = 0;
+    for (int i0 = 0; i0 < V; i0 += kGroup) {
+        unsigned long long mine = 0;
+#pragma unroll
+        for (int h = 0; h < kGroupSteps; h += 8) {
+            float v[8];
+            load_steps(x, i0 + h * kFinishThreads + tid, kFinishThreads, V, v);
+#pragma unroll
+            for (int j = 0; j < 8; j++) mine += whole(weight_at(v[j], i0 + (h + j) * kFinishThreads + tid));
+        }
+        const unsigned long long group = block_sum_u64(mine, red);
+        if (tid == 0) list[i0 / kGroup] = group;
+        total += group;
+    }
+    __syncthreads();
+    const double u = fmin(fmax(a.u[r], 0.0), 1.0);          // NaN: 0
+    unsigned long long goal = (unsigned long long)floor(u * (double)total);      // the first token with (running weight) > goal
+    if (goal >= total) goal = total - 1;
+    unsigned long long before = 0;
+    int i0 = 0;
+    while (before + list[i0 / kGroup] <= goal) {
+        before += list[i0 / kGroup];
+        i0 += kGroup;
+    }
+    for (int s = 0; s < kGroupSteps; s++, i0 += kFinishThreads) {
+        const double f = i0 + tid < V ? weight_at(x[i0 + tid], i0 + tid) : 0.0;
+        const unsigned long long mine = whole(f);
+        unsigned long long step;
+        const unsigned long long at = before + block_scan_u64(mine, red, step);
+        if (mine && at <= goal && goal < at + mine) {
+            a.out_token[r] = i0 + tid;
+            if (a.out_prob) a.out_prob[r] = (float)(f / (double)total);
+        }
+        before += step;
+        if (before > goal) break;                           // the same for every thread
+    }
+}
+
 }  // namespace
 }  // namespace rt
 
 using rt::fail;
 using rt::Guard;
+using rt::ensure_scratch;
 
 extern "C" {
 
@@ -202,8 +573,26 @@ int rt_hip_sample_dev(rt_hip_ctx *ctx, const float *logits, size_t ld, int n_row
     Guard g(ctx);
     int bits = 0;
     while ((1 << bits) < vocab) bits++;
-    rt::SampleArgs a{ logits, ld, n_rows, vocab, bits < 10 ? 52 : 62 - bits, u, temperature, top_p, min_p, top_k, out_token, out_prob };
-    rt::sample_kernel<<<dim3((unsigned)n_rows), rt::kSampleThreads, 0, ctx->stream>>>(a);
+    rt::SampleArgs a{ logits, ld, n_rows, vocab, bits < 11 ? 51 : 62 - bits, u, temperature, top_p, min_p, top_k, out_token, out_prob };
+    // a row is split so that about a thousand workgroups share the first two launches, 2048 tokens at least in each; rows go in
+    // groups whose histograms stay below 16 MB
+    const int group = std::min(n_rows, 1024);
+    rt::SampleWork w;
+    w.splits = std::max(1, std::min(1024 / group, (vocab + 2047) / 2048));
+    w.per_split = (vocab + w.splits - 1) / w.splits;
+    const size_t bins = (size_t)group * rt::kBins;
+    int rc = ensure_scratch(ctx, bins * 12 + (size_t)group * w.splits * sizeof(rt::RowRange));
+    if (rc) return rc;
+    w.sum = static_cast<unsigned long long *>(ctx->scratch);
+    w.count = reinterpret_cast<uint32_t *>(w.sum + bins);
+    w.range = reinterpret_cast<rt::RowRange *>(w.count + bins);
+    for (w.row0 = 0; w.row0 < n_rows; w.row0 += group) {
+        const int rows = std::min(group, n_rows - w.row0);
+        const dim3 grid((unsigned)w.splits, (unsigned)rows);
+        rt::sample_range_kernel<<<grid, 256, 0, ctx->stream>>>(a, w);
+        rt::sample_histogram_kernel<<<grid, 256, 0, ctx->stream>>>(a, w);
+        rt::sample_finish_kernel<<<dim3((unsigned)rows), rt::kFinishThreads, 0, ctx->stream>>>(a, w);
+    }
     RT_TRY_HIP(ctx, hipGetLastError());
     return RT_HIP_OK;
 }

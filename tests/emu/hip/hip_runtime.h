@@ -280,6 +280,7 @@ inline short emu_bload16(emu_buffer_rsrc r, unsigned voff, unsigned soff) { shor
 // ---- device-scope atomics: fibers never run concurrently, so any access would be exact; they go through the
 // compiler's atomics so that the race detector of the ThreadSanitizer build knows them for what they are
 #define __HIP_MEMORY_SCOPE_AGENT 0
+#define __HIP_MEMORY_SCOPE_WORKGROUP 0
 template <class T> inline T emu_atomic_load(const T *p) { T v; __atomic_load(p, &v, __ATOMIC_RELAXED); return v; }
 template <class T> inline void emu_atomic_store(T *p, T v) { __atomic_store(p, &v, __ATOMIC_RELAXED); }
 template <class T> inline T emu_fetch_add(T *p, T v) { return __atomic_fetch_add(p, v, __ATOMIC_RELAXED); }
