@@ -10,10 +10,10 @@
 // the draw do not depend on how the row is split over threads, and a token is lost to rounding only below 2^-(F+1) of the
 // largest weight (F = 45 for a vocabulary of 131072).  32-bit sums would move the cuts of a large vocabulary by whole tokens.
 //
-// Three launches: sample_range_kernel finds each row's largest logit (and its smallest finite one), sample_histogram_kernel
-// counts and weighs the tokens by how far below it they are, both with a row split over as many workgroups as fill the device;
-// sample_finish_kernel, one workgroup per row, finds from the histogram the bins that the cuts fall into, ranks the tokens of
-// just those bins exactly, and draws.
+// Four launches.  sample_range_kernel finds each row's largest logit (and its smallest finite one), sample_histogram_kernel counts
+// and weighs the tokens by how far below it they are, sample_collect_kernel finds from the histogram the bins that the cuts fall
+// into, lists the tokens of just those bins and sums the weights of the tokens above them, sample_finish_kernel ranks the listed
+// tokens exactly and draws.  The first three split a row over as many workgroups as fill the device.
 #include "rt_device.h"
 
 #include <algorithm>
@@ -69,21 +69,40 @@ __device__ __forceinline__ unsigned long long block_sum_u64(unsigned long long v
 
 // ---- bins: a row's tokens by their distance d = M - l below the largest logit, up to the distance R beyond which the weight
 // rounds to zero (or the smallest finite logit, if that is nearer): the bin's number is floor(d * (kBins - 1) / R), which is
-// monotone in d.  The weight of a token is the weight of its bin's middle, from a table, times exp(-r), |r| <= 0.016, by its
-// series to the sixth power (the next term is below 2^-54): a dozen 64-bit operations where exp() takes four times as many.
-// The middle is the same rounded number in the table and in r, and so the product is as exact as exp() itself.
-constexpr int kBins = 1024, kFinishThreads = 1024, kListMost = 2048, kGroupSteps = 16;
+// monotone in d.  The weight of a token is the weight at the middle of its kTable-th part of the reach, from a table, times
+// exp(-r), |r| <= 0.016, by its series to the sixth power (the next term is below 2^-54): a dozen 64-bit operations where exp()
+// takes four times as many.  The middle is the same rounded number in the table and in r, and so the product is as exact as
+// exp() itself.
+// 4096 bins hold at most a few dozen tokens each where the cuts of real rows fall; 1024 held hundreds, whose ranking (every one
+// against every other) took most of the time.
+constexpr int kBins = 4096, kTable = 1024, kThreads = 256, kCountThreads = 512, kListMost = 2048, kPart = 4096;
 
 struct RowRange { float top, low; int arg, pad; };        // of one split of a row: largest logit, smallest finite one, index of the largest
+// What the histogram says of a row's cuts.
+struct RowBorders {
+    unsigned long long all;                                // weight of the row
+    unsigned long long k_weight_above, k_weight_with;      // above the bin that top-k ends in, and with it
+    unsigned long long k_above, k_in;                      // tokens above that bin and in it
+    unsigned long long k;                                  // top-k, 0 where it keeps every token that weighs anything
+    unsigned long long above_list;                         // weight above the first listed bin of top-p
+    int k_bin;                                             // kBins: no top-k
+    int p_first, p_last;                                   // the bins that top-p may end in (p_last = -1: no top-p)
+    int keep_below;                                        // bins below this one stay whole
+};
 struct SampleWork {
     RowRange *range;                                       // [row][split]
     unsigned long long *sum;                               // [row][kBins]
     uint32_t *count;                                       // [row][kBins]
-    int row0, splits, per_split;                           // this launch's first row
+    RowBorders *borders;                                   // [row]
+    int *listed;                                           // [row]: tokens listed
+    unsigned long long *list;                              // [row][kListMost]: their keys
+    unsigned long long *part_sum;                          // [row][part]: weight that stays whole, of kPart tokens each
+    int row0, splits, per_split, parts;                    // this launch's first row
 };
 
 struct RowBins {
-    double top, scale, width, inv_t;
+    double top, scale, inv_t;
+    double width;                 // of a table entry
     float topf;
 };
 __device__ __forceinline__ RowBins row_bins(float top, float low, double T, int frac_bits) {
@@ -93,28 +112,31 @@ __device__ __forceinline__ RowBins row_bins(float top, float low, double T, int 
     b.topf = top;
     b.top = (double)top;
     b.scale = R > 0.0 ? (double)(kBins - 1) / R : 0.0;
-    b.width = R / (double)(kBins - 1);
+    b.width = R / (double)(kBins - 1) * (double)(kBins / kTable);
     b.inv_t = 1.0 / T;
     return b;
 }
 #pragma clang fp contract(off)
-__device__ __forceinline__ double bin_middle(const RowBins &b, int bin) { return ((double)bin + 0.5) * b.width; }
+__device__ __forceinline__ double entry_middle(const RowBins &b, int entry) { return ((double)entry + 0.5) * b.width; }
 __device__ __forceinline__ int bin_of(const RowBins &b, float x) {       // kBins: beyond the reach, NaN or infinite
     const double at = (b.top - (double)x) * b.scale;
     return at < (double)kBins ? (int)at : kBins;                         // false for NaN
 }
-__device__ __forceinline__ double table_entry(const RowBins &b, int bin, int frac_bits) { return ldexp(exp(-(bin_middle(b, bin) * b.inv_t)), frac_bits); }
+__device__ __forceinline__ void fill_table(const RowBins &b, int frac_bits, double *table) {
+    for (int i = threadIdx.x; i < kTable; i += blockDim.x) table[i] = ldexp(exp(-(entry_middle(b, i) * b.inv_t)), frac_bits);
+}
 // the weight times 2^frac_bits
 __device__ __forceinline__ double binned_weight(const RowBins &b, float x, int bin, const double *table, int frac_bits) {
     if (x == b.topf) return ldexp(1.0, frac_bits);
-    const double r = ((b.top - (double)x) - bin_middle(b, bin)) * -b.inv_t;
+    const int entry = bin / (kBins / kTable);
+    const double r = ((b.top - (double)x) - entry_middle(b, entry)) * -b.inv_t;
     double e = fma(r, 1.0 / 720.0, 1.0 / 120.0);
     e = fma(e, r, 1.0 / 24.0);
     e = fma(e, r, 1.0 / 6.0);
     e = fma(e, r, 0.5);
     e = fma(e, r, 1.0);
     e = fma(e, r, 1.0);
-    return table[bin] * e;
+    return table[entry] * e;
 }
 __device__ __forceinline__ unsigned long long whole(double w) {          // rounded to nearest, 0 <= w <= 2^51: the sum's last bits
     return __builtin_bit_cast(unsigned long long, w + 4503599627370496.0) - 0x4330000000000000ull;
@@ -148,7 +170,7 @@ __device__ __forceinline__ void load_steps(const float *x, int i, int step, int 
 }
 
 // The range of one split of a row; also clears the split's share of the row's histogram.
-__global__ __launch_bounds__(256) void sample_range_kernel(SampleArgs a, SampleWork w) {
+__global__ __launch_bounds__(kThreads) void sample_range_kernel(SampleArgs a, SampleWork w) {
     __shared__ float tops[4], lows[4];
     __shared__ int args[4];
     const int tid = threadIdx.x, split = blockIdx.x, row = blockIdx.y, r = w.row0 + row;
@@ -180,6 +202,7 @@ __global__ __launch_bounds__(256) void sample_range_kernel(SampleArgs a, SampleW
         }
         w.range[(size_t)row * w.splits + split] = RowRange{ top, low, arg, 0 };
     }
+    if (split == 0 && tid == 0) w.listed[row] = 0;
     const int share = (kBins + w.splits - 1) / w.splits, b1 = min(kBins, (split + 1) * share);
     for (int b = split * share + tid; b < b1; b += 256) {
         w.sum[(size_t)row * kBins + b] = 0;
@@ -204,39 +227,41 @@ __device__ __forceinline__ RowRange row_range(const SampleWork &w, int row) {
     return g;
 }
 
-__global__ __launch_bounds__(256) void sample_histogram_kernel(SampleArgs a, SampleWork w) {
-    __shared__ double table[kBins];
+__global__ __launch_bounds__(kCountThreads) void sample_histogram_kernel(SampleArgs a, SampleWork w) {
+    __shared__ double table[kTable];
     __shared__ unsigned long long sum[kBins];
     __shared__ uint32_t count[kBins];
     const int tid = threadIdx.x, split = blockIdx.x, row = blockIdx.y, r = w.row0 + row;
     const float *x = a.logits + (size_t)r * a.ld;
     const RowAsks q = row_asks(a, r);
+    if (q.greedy || !(q.k > 0 || q.p > 0.f)) return;                      // no cut to find
     const RowRange g = row_range(w, row);
-    if (q.greedy || g.top == -INFINITY || g.top == INFINITY) return;      // decided by the range alone, or without weights
+    if (g.top == -INFINITY || g.top == INFINITY) return;                  // without weights
+    const bool weighs = q.p > 0.f;                                        // top-k alone counts
     const RowBins b = row_bins(g.top, g.low, q.T, a.frac_bits);
-    for (int i = tid; i < kBins; i += 256) {
-        table[i] = table_entry(b, i, a.frac_bits);
+    if (weighs) fill_table(b, a.frac_bits, table);
+    for (int i = tid; i < kBins; i += kCountThreads) {
         sum[i] = 0;
         count[i] = 0;
     }
     __syncthreads();
     const int i0 = split * w.per_split, i1 = min(a.vocab, i0 + w.per_split);
-    for (int i = i0 + tid; i < i1; i += 8 * 256) {
+    for (int i = i0 + tid; i < i1; i += 8 * kCountThreads) {
         float v[8];
-        load_steps(x, i, 256, i1, v);
+        load_steps(x, i, kCountThreads, i1, v);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int bin = bin_of(b, v[j]);
             if (bin < kBins) {
-                __hip_atomic_fetch_add(&sum[bin], whole(binned_weight(b, v[j], bin, table, a.frac_bits)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                if (weighs) __hip_atomic_fetch_add(&sum[bin], whole(binned_weight(b, v[j], bin, table, a.frac_bits)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                 __hip_atomic_fetch_add(&count[bin], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             }
         }
     }
     __syncthreads();
-    for (int i = tid; i < kBins; i += 256)
+    for (int i = tid; i < kBins; i += kCountThreads)
         if (count[i]) {
-            __hip_atomic_fetch_add(&w.sum[(size_t)row * kBins + i], sum[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (weighs) __hip_atomic_fetch_add(&w.sum[(size_t)row * kBins + i], sum[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             __hip_atomic_fetch_add(&w.count[(size_t)row * kBins + i], count[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
 }
@@ -265,9 +290,118 @@ __device__ __forceinline__ unsigned long long block_scan_u64(unsigned long long 
     return before + s - v;
 }
 
+// The cuts' bins, from the row's histogram; the whole workgroup calls this and gets the answer in `out` (LDS).
+__device__ void find_borders(const SampleWork &w, int row, const RowAsks &q, unsigned long long *red, RowBorders &out) {
+    constexpr int kOwn = kBins / kThreads;
+    const int tid = threadIdx.x;
+    unsigned long long sum[kOwn], sums = 0, counts = 0, all_weight, all_tokens;
+    uint32_t count[kOwn];
+#pragma unroll
+    for (int j = 0; j < kOwn; j++) {
+        sum[j] = w.sum[(size_t)row * kBins + tid * kOwn + j];
+        count[j] = w.count[(size_t)row * kBins + tid * kOwn + j];
+    }
+#pragma unroll
+    for (int j = 0; j < kOwn; j++) {
+        sums += sum[j];
+        counts += count[j];
+    }
+    const unsigned long long n0 = block_scan_u64(counts, red, all_tokens), s0 = block_scan_u64(sums, red, all_weight);
+    const unsigned long long k = q.k > 0 && (unsigned long long)q.k < all_tokens ? (unsigned long long)q.k : 0;
+    if (tid == 0) out = RowBorders{ all_weight, all_weight, all_weight, 0, 0, k, 0, kBins, 0, -1, kBins };
+    __syncthreads();
+    if (k) {
+        unsigned long long n = n0, s = s0;
+#pragma unroll
+        for (int j = 0; j < kOwn; j++) {
+            if (n < k && k <= n + count[j]) {
+                out.k_bin = tid * kOwn + j;
+                out.k_weight_above = s;
+                out.k_weight_with = s + sum[j];
+                out.k_above = n;
+                out.k_in = count[j];
+            }
+            n += count[j];
+            s += sum[j];
+        }
+        __syncthreads();
+    }
+    if (q.p > 0.f) {
+        // the weight of the top k lies between that of the bins above its last one and that with it
+        const double lo = (double)q.p * (double)out.k_weight_above, hi = (double)q.p * (double)out.k_weight_with;
+        unsigned long long s = s0;
+#pragma unroll
+        for (int j = 0; j < kOwn; j++) {
+            const double from = (double)s, to = (double)(s + sum[j]);
+            if (sum[j] && from < lo && lo <= to) {
+                out.p_first = tid * kOwn + j;               // stays 0 where nothing lies above the bin of top-k
+                out.above_list = s;
+            }
+            if (sum[j] && from < hi && hi <= to) out.p_last = tid * kOwn + j;
+            s += sum[j];
+        }
+    }
+    __syncthreads();
+    if (tid == 0) out.keep_below = q.p > 0.f ? out.p_first : out.k_bin;
+    __syncthreads();
+}
+
+// One workgroup per kPart tokens of a row: lists the tokens of the cuts' bins and sums the weights of the tokens above them.
+__global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a, SampleWork w) {
+    __shared__ double table[kTable];
+    __shared__ unsigned long long found[kListMost], red[kThreads / 64];
+    __shared__ RowBorders borders;
+    __shared__ int n_found, place;
+    const int tid = threadIdx.x, part = blockIdx.x, row = blockIdx.y, r = w.row0 + row;
+    const float *x = a.logits + (size_t)r * a.ld;
+    const RowAsks q = row_asks(a, r);
+    if (q.greedy) return;
+    const RowRange g = row_range(w, row);
+    if (g.top == -INFINITY || g.top == INFINITY) return;
+    const RowBins b = row_bins(g.top, g.low, q.T, a.frac_bits);
+    fill_table(b, a.frac_bits, table);
+    if (tid == 0) n_found = 0;
+    if (q.k > 0 || q.p > 0.f) {
+        find_borders(w, row, q, red, borders);
+    } else {
+        if (tid == 0) borders = RowBorders{ 0, 0, 0, 0, 0, 0, 0, kBins, 0, -1, kBins };
+        __syncthreads();
+    }
+    if (part == 0 && tid == 0) w.borders[row] = borders;
+    const int k_bin = borders.k_bin, p_first = borders.p_first, p_last = borders.p_last, keep_below = borders.keep_below;
+    const double min_w = ldexp(q.min_w, a.frac_bits);
+    const int i0 = part * kPart, i1 = min(a.vocab, i0 + kPart);
+    unsigned long long mine = 0;
+    for (int i = i0 + tid; i < i1; i += 8 * kThreads) {
+        float v[8];
+        load_steps(x, i, kThreads, i1, v);
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const int bin = bin_of(b, v[j]);
+            if (bin >= kBins) continue;
+            if (bin < keep_below) {
+                const double f = binned_weight(b, v[j], bin, table, a.frac_bits);
+                if (f >= min_w) mine += whole(f);
+            } else if (bin == k_bin || (bin >= p_first && bin <= p_last)) {
+                const int at = __hip_atomic_fetch_add(&n_found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                if (at < kListMost) found[at] = rank_key(v[j], i + j * kThreads);
+            }
+        }
+    }
+    mine = block_sum_u64(mine, red);                        // its barriers also publish the list
+    if (tid == 0) {
+        w.part_sum[(size_t)row * w.parts + part] = mine;
+        place = n_found ? __hip_atomic_fetch_add(&w.listed[row], n_found, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
+    }
+    __syncthreads();
+    const int at = place, n = min(n_found, kListMost);      // more than the list holds: the count says so
+    for (int i = tid; i < n; i += kThreads)
+        if (at + i < kListMost) w.list[(size_t)row * kListMost + at + i] = found[i];
+}
+
 // The row on its own, without bins: the cuts by bisection over the 32 bits of the logits' order, one pass over the row per bit.
 // For rows with infinite logits and for rows with more equal or nearly equal logits in one bin than the list of
-// sample_finish_kernel holds.  run: kFinishThreads entries, tie as many.
+// sample_finish_kernel holds.  run: kThreads entries, tie as many.
 __device__ void sample_by_bisection(const SampleArgs &a, int r, const RowAsks &q, float top, unsigned long long *run, int *tie, unsigned long long *red) {
     const int tid = threadIdx.x, V = a.vocab, k = q.k > 0 ? q.k : V;
     const float *x = a.logits + (size_t)r * a.ld;
@@ -278,12 +412,12 @@ __device__ void sample_by_bisection(const SampleArgs &a, int r, const RowAsks &q
     // ---- the cut: tokens above `cut` stay, of those at `cut` the first `ties` by index
     auto count_from = [&](uint32_t o) {              // tokens at o or above
         unsigned long long n = 0;
-        for (int i = tid; i < V; i += kFinishThreads) n += logit_order(x[i]) >= o ? 1 : 0;
+        for (int i = tid; i < V; i += kThreads) n += logit_order(x[i]) >= o ? 1 : 0;
         return block_sum_u64(n, red);
     };
     auto weight_from = [&](uint32_t o) {
         unsigned long long n = 0;
-        for (int i = tid; i < V; i += kFinishThreads)
+        for (int i = tid; i < V; i += kThreads)
             if (logit_order(x[i]) >= o) n += fixed_weight(x[i], top, T, a.frac_bits);
         return block_sum_u64(n, red);
     };
@@ -328,7 +462,7 @@ __device__ void sample_by_bisection(const SampleArgs &a, int r, const RowAsks &q
     }
 
     // ---- the draw, by index: each thread owns consecutive tokens
-    const int per = (V + kFinishThreads - 1) / kFinishThreads, i0 = min(V, tid * per), i1 = min(V, i0 + per);
+    const int per = (V + kThreads - 1) / kThreads, i0 = min(V, tid * per), i1 = min(V, i0 + per);
     int mine = 0;
     for (int i = i0; i < i1; i++) mine += logit_order(x[i]) == cut ? 1 : 0;
     tie[tid] = mine;
@@ -347,7 +481,7 @@ __device__ void sample_by_bisection(const SampleArgs &a, int r, const RowAsks &q
     run[tid] = sum;
     __syncthreads();
     unsigned long long total = 0, before = 0;
-    for (int j = 0; j < kFinishThreads; j++) {
+    for (int j = 0; j < kThreads; j++) {
         if (j == tid) before = total;
         total += run[j];
     }
@@ -370,14 +504,14 @@ __device__ void sample_by_bisection(const SampleArgs &a, int r, const RowAsks &q
     }
 }
 
-__global__ __launch_bounds__(kFinishThreads) void sample_finish_kernel(SampleArgs a, SampleWork w) {
-    static_assert(kBins == kFinishThreads && kListMost % kFinishThreads == 0, "a thread owns a bin and so many places of the list");
-    constexpr int kMine = kListMost / kFinishThreads, kGroup = kGroupSteps * kFinishThreads;
-    __shared__ double table[kBins];
-    // keys and weights of the tokens in the bins that the cuts fall into
-    __shared__ unsigned long long list[kListMost], list_weight[kListMost];
-    __shared__ unsigned long long red[kFinishThreads / 64], shared64[6];
-    __shared__ int listed, shared32[4];
+__global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, SampleWork w) {
+    constexpr int kMine = kListMost / kThreads, kOwn = kPart / kThreads;
+    __shared__ double table[kTable];
+    __shared__ unsigned long long buf[kPart];               // the list's keys and weights; the weights of one part; bisection's scratch
+    __shared__ unsigned long long red[kThreads / 64], shared64[2];
+    __shared__ int chosen;
+    static_assert(2 * kListMost <= kPart && kOwn <= kThreads, "the list fits the buffer");
+    unsigned long long *list = buf, *list_weight = buf + kListMost;
     const int tid = threadIdx.x, row = blockIdx.x, r = w.row0 + row, V = a.vocab;
     const float *x = a.logits + (size_t)r * a.ld;
     const RowAsks q = row_asks(a, r);
@@ -389,168 +523,131 @@ __global__ __launch_bounds__(kFinishThreads) void sample_finish_kernel(SampleArg
         }
         return;
     }
-    if (g.top == INFINITY) {
-        sample_by_bisection(a, r, q, g.top, list, reinterpret_cast<int *>(list_weight), red);
+    const int n_list = g.top == INFINITY ? 0 : w.listed[row];
+    if (g.top == INFINITY || n_list > kListMost) {
+        sample_by_bisection(a, r, q, g.top, buf, reinterpret_cast<int *>(buf + kThreads), red);
         return;
     }
     const RowBins b = row_bins(g.top, g.low, q.T, a.frac_bits);
-    table[tid] = table_entry(b, tid, a.frac_bits);
+    const RowBorders c = w.borders[row];
+    const double min_w = ldexp(q.min_w, a.frac_bits);
+    fill_table(b, a.frac_bits, table);
+    __syncthreads();
 
     // ---- the last key that stays
     unsigned long long cut = ~0ull;
-    if (q.k > 0 || q.p > 0.f) {
-        const unsigned long long bin_sum = w.sum[(size_t)row * kBins + tid], bin_count = w.count[(size_t)row * kBins + tid];
-        unsigned long long n_all, s_all;
-        const unsigned long long n_before = block_scan_u64(bin_count, red, n_all), s_before = block_scan_u64(bin_sum, red, s_all);
-        const unsigned long long k = q.k > 0 && (unsigned long long)q.k < n_all ? (unsigned long long)q.k : 0;
-        if (tid == 0) {
-            listed = 0;
-            shared32[0] = kBins;                            // the bin that top-k ends in (kBins: none)
-            shared64[0] = shared64[1] = s_all;              // weight above that bin, weight with it
-            shared64[2] = shared64[3] = 0;                  // tokens above it, tokens in it
-            shared32[1] = 0;                                // first and last bin that top-p may end in
-            shared32[2] = -1;
-        }
-        __syncthreads();
-        if (k && n_before < k && k <= n_before + bin_count) {
-            shared32[0] = tid;
-            shared64[0] = s_before;
-            shared64[1] = s_before + bin_sum;
-            shared64[2] = n_before;
-            shared64[3] = bin_count;
-        }
-        __syncthreads();
-        const int k_bin = shared32[0];
-        const unsigned long long k_weight_above = shared64[0], k_above = shared64[2], k_in = shared64[3];
-        if (q.p > 0.f && bin_sum) {
-            // the weight of the top k lies between that of the bins above its last one and that with it
-            const double lo = (double)q.p * (double)k_weight_above, hi = (double)q.p * (double)shared64[1];
-            const double from = (double)s_before, to = (double)(s_before + bin_sum);
-            if (from < lo && lo <= to) shared32[1] = tid;
-            if (from < hi && hi <= to) shared32[2] = tid;
-        }
-        if (tid == 0) shared64[4] = 0;
-        __syncthreads();
-        const int p_first = shared32[1], p_last = shared32[2];
-        if (tid == p_first) shared64[5] = s_before;         // weight above the bins of top-p, read behind the next barrier
-        for (int i0 = tid; i0 < V; i0 += 8 * kFinishThreads) {
-            float v[8];
-            load_steps(x, i0, kFinishThreads, V, v);
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int bin = bin_of(b, v[j]);
-                if (bin < kBins && (bin == k_bin || (bin >= p_first && bin <= p_last))) {
-                    const int at = __hip_atomic_fetch_add(&listed, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                    if (at < kListMost) {
-                        list[at] = rank_key(v[j], i0 + j * kFinishThreads);
-                        list_weight[at] = whole(binned_weight(b, v[j], bin, table, a.frac_bits));
-                    }
-                }
-            }
-        }
-        __syncthreads();
-        const int n_list = listed;
-        if (n_list > kListMost) {
-            sample_by_bisection(a, r, q, g.top, list, reinterpret_cast<int *>(list_weight), red);
-            return;
-        }
-        // ---- every listed token's number and weight of listed tokens before it.  The listed bins are top-p's, one after the
-        // other, and top-k's, which is the last of them or comes behind them.
-        unsigned long long key[kMine], own[kMine], weight_before[kMine];
+    unsigned long long key[kMine], own[kMine];
+    if (n_list > 0) {
+        unsigned long long weight_before[kMine];
         int rank[kMine];
 #pragma unroll
         for (int m = 0; m < kMine; m++) {
-            const int i = tid + m * kFinishThreads;
-            key[m] = i < n_list ? list[i] : 0;
-            own[m] = i < n_list ? list_weight[i] : 0;
-            weight_before[m] = 0;
+            const int i = tid + m * kThreads;
+            key[m] = own[m] = weight_before[m] = 0;
             rank[m] = 0;
+            if (i < n_list) {
+                key[m] = w.list[(size_t)row * kListMost + i];
+                const float v = order_logit(~(uint32_t)(key[m] >> 32));
+                own[m] = whole(binned_weight(b, v, bin_of(b, v), table, a.frac_bits));
+                list[i] = key[m];
+                list_weight[i] = own[m];
+            }
         }
+        __syncthreads();
+        // every listed token's number and weight of listed tokens before it.  The listed bins are top-p's, one after the other, and
+        // top-k's, which is the last of them or comes behind them.
         for (int j = 0; j < n_list; j++) {
             const unsigned long long other = list[j], its = list_weight[j];
 #pragma unroll
             for (int m = 0; m < kMine; m++)
-                if (other < key[m]) {
+                if (m * kThreads < n_list && other < key[m]) {
                     rank[m]++;
                     weight_before[m] += its;
                 }
         }
-        const unsigned long long above_list = shared64[5];
-        double goal = (double)q.p * (double)s_all;
-        if (k) {
+        double goal = (double)q.p * (double)c.all;
+        if (c.k) {
             unsigned long long mine = 0;
-            const int k_from = n_list - (int)k_in;          // where the list's part in the bin of top-k begins
+            const int k_from = n_list - (int)c.k_in;        // where the list's part in the bin of top-k begins
 #pragma unroll
             for (int m = 0; m < kMine; m++)
-                if (tid + m * kFinishThreads < n_list && rank[m] >= k_from) {
-                    const unsigned long long nth = k_above + (unsigned long long)(rank[m] - k_from);
-                    if (nth < k) mine += own[m];
-                    if (nth == k - 1) shared64[4] = key[m];
+                if (tid + m * kThreads < n_list && rank[m] >= k_from) {
+                    const unsigned long long nth = c.k_above + (unsigned long long)(rank[m] - k_from);
+                    if (nth < c.k) mine += own[m];
+                    if (nth == c.k - 1) shared64[0] = key[m];
                 }
-            mine = block_sum_u64(mine, red);                // its barriers publish shared64[4]
-            cut = shared64[4];
-            goal = (double)q.p * (double)(k_weight_above + mine);
+            mine = block_sum_u64(mine, red);                // its barriers publish shared64[0]
+            cut = shared64[0];
+            goal = (double)q.p * (double)(c.k_weight_above + mine);
         }
         if (q.p > 0.f) {
             // the first token at which the weight reaches the goal; it is one of the listed, and not behind top-k's last
 #pragma unroll
             for (int m = 0; m < kMine; m++)
-                if (tid + m * kFinishThreads < n_list && key[m] <= cut) {
-                    const unsigned long long before = above_list + weight_before[m];
-                    if ((double)before < goal && (double)(before + own[m]) >= goal) shared64[0] = key[m];
+                if (tid + m * kThreads < n_list && key[m] <= cut) {
+                    const unsigned long long before = c.above_list + weight_before[m];
+                    if ((double)before < goal && (double)(before + own[m]) >= goal) shared64[1] = key[m];
                 }
             __syncthreads();
-            cut = shared64[0];
+            cut = shared64[1];
         }
+        __syncthreads();                                    // the list's memory is free from here on
     }
-    __syncthreads();                                        // the table; the list is free from here on
 
-    // ---- the draw, by index, over the tokens whose key is at most the cut: the group of kGroup tokens, then the step of the
-    // group, then the wave and the lane
-    const double min_w = ldexp(q.min_w, a.frac_bits);
-    auto weight_at = [&](float v, int i) -> double {        // 0: not kept; kept weights are whole()d by the caller
-        if (rank_key(v, i) > cut) return 0.0;
-        const int bin = bin_of(b, v);
-        if (bin >= kBins) return 0.0;
-        const double f = binned_weight(b, v, bin, table, a.frac_bits);
-        return f >= min_w ? f : 0.0;
-    };
-    unsigned long long total = 0;
-    for (int i0 = 0; i0 < V; i0 += kGroup) {
-        unsigned long long mine = 0;
-#pragma unroll
-        for (int h = 0; h < kGroupSteps; h += 8) {
-            float v[8];
-            load_steps(x, i0 + h * kFinishThreads + tid, kFinishThreads, V, v);
-#pragma unroll
-            for (int j = 0; j < 8; j++) mine += whole(weight_at(v[j], i0 + (h + j) * kFinishThreads + tid));
-        }
-        const unsigned long long group = block_sum_u64(mine, red);
-        if (tid == 0) list[i0 / kGroup] = group;
-        total += group;
-    }
+    // ---- the draw, by index, over the tokens whose key is at most the cut: which part, then which token of it.  What stays of the
+    // listed tokens joins the parts' sums first.
+    for (int p = tid; p < w.parts; p += kThreads) buf[p] = w.part_sum[(size_t)row * w.parts + p];
     __syncthreads();
+    if (n_list > 0) {
+#pragma unroll
+        for (int m = 0; m < kMine; m++)
+            if (tid + m * kThreads < n_list && key[m] <= cut) {
+                const float v = order_logit(~(uint32_t)(key[m] >> 32));
+                if (binned_weight(b, v, bin_of(b, v), table, a.frac_bits) >= min_w)
+                    __hip_atomic_fetch_add(&buf[(uint32_t)key[m] / kPart], own[m], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            }
+        __syncthreads();
+    }
+    unsigned long long total;
+    const unsigned long long part = tid < w.parts ? buf[tid] : 0, before_part = block_scan_u64(part, red, total);      // at most kThreads parts
     const double u = fmin(fmax(a.u[r], 0.0), 1.0);          // NaN: 0
     unsigned long long goal = (unsigned long long)floor(u * (double)total);      // the first token with (running weight) > goal
     if (goal >= total) goal = total - 1;
-    unsigned long long before = 0;
-    int i0 = 0;
-    while (before + list[i0 / kGroup] <= goal) {
-        before += list[i0 / kGroup];
-        i0 += kGroup;
+    if (part && before_part <= goal && goal < before_part + part) {
+        chosen = tid;
+        shared64[0] = before_part;
     }
-    for (int s = 0; s < kGroupSteps; s++, i0 += kFinishThreads) {
-        const double f = i0 + tid < V ? weight_at(x[i0 + tid], i0 + tid) : 0.0;
-        const unsigned long long mine = whole(f);
-        unsigned long long step;
-        const unsigned long long at = before + block_scan_u64(mine, red, step);
-        if (mine && at <= goal && goal < at + mine) {
-            a.out_token[r] = i0 + tid;
-            if (a.out_prob) a.out_prob[r] = (float)(f / (double)total);
+    __syncthreads();
+    const int i0 = chosen * kPart;
+    unsigned long long before = shared64[0];
+    float v[kOwn];
+    load_steps(x, i0 + tid, kThreads, V, v);
+#pragma unroll
+    for (int j = 0; j < kOwn; j++) {
+        const int i = i0 + j * kThreads + tid, bin = bin_of(b, v[j]);
+        unsigned long long weight = 0;
+        if (bin < kBins && rank_key(v[j], i) <= cut) {
+            const double f = binned_weight(b, v[j], bin, table, a.frac_bits);
+            if (f >= min_w) weight = whole(f);
         }
-        before += step;
-        if (before > goal) break;                           // the same for every thread
+        buf[j * kThreads + tid] = weight;
     }
+    __syncthreads();
+    // a thread per kOwn consecutive tokens
+    unsigned long long mine = 0, sum;
+    for (int j = 0; j < kOwn; j++) mine += buf[tid * kOwn + j];
+    unsigned long long at = before + block_scan_u64(mine, red, sum);
+    if (mine && at <= goal && goal < at + mine)
+        for (int j = 0; j < kOwn; j++) {
+            const unsigned long long weight = buf[tid * kOwn + j];
+            if (weight && goal < at + weight) {
+                const int i = i0 + tid * kOwn + j;
+                a.out_token[r] = i;
+                if (a.out_prob) a.out_prob[r] = (float)(binned_weight(b, x[i], bin_of(b, x[i]), table, a.frac_bits) / (double)total);
+                break;
+            }
+            at += weight;
+        }
 }
 
 }  // namespace
@@ -575,23 +672,29 @@ int rt_hip_sample_dev(rt_hip_ctx *ctx, const float *logits, size_t ld, int n_row
     while ((1 << bits) < vocab) bits++;
     rt::SampleArgs a{ logits, ld, n_rows, vocab, bits < 11 ? 51 : 62 - bits, u, temperature, top_p, min_p, top_k, out_token, out_prob };
     // a row is split so that about a thousand workgroups share the first two launches, 2048 tokens at least in each; rows go in
-    // groups whose histograms stay below 16 MB
+    // groups whose histograms stay below 64 MB
     const int group = std::min(n_rows, 1024);
     rt::SampleWork w;
     w.splits = std::max(1, std::min(1024 / group, (vocab + 2047) / 2048));
     w.per_split = (vocab + w.splits - 1) / w.splits;
-    const size_t bins = (size_t)group * rt::kBins;
-    int rc = ensure_scratch(ctx, bins * 12 + (size_t)group * w.splits * sizeof(rt::RowRange));
+    w.parts = (vocab + rt::kPart - 1) / rt::kPart;
+    const size_t bins = (size_t)group * rt::kBins, list = (size_t)group * rt::kListMost, parts = (size_t)group * w.parts;
+    int rc = ensure_scratch(ctx, (bins + list + parts) * 8 + group * sizeof(rt::RowBorders) + (size_t)group * w.splits * sizeof(rt::RowRange) + bins * 4 + (size_t)group * 4);
     if (rc) return rc;
     w.sum = static_cast<unsigned long long *>(ctx->scratch);
-    w.count = reinterpret_cast<uint32_t *>(w.sum + bins);
-    w.range = reinterpret_cast<rt::RowRange *>(w.count + bins);
+    w.list = w.sum + bins;
+    w.part_sum = w.list + list;
+    w.borders = reinterpret_cast<rt::RowBorders *>(w.part_sum + parts);
+    w.range = reinterpret_cast<rt::RowRange *>(w.borders + group);
+    w.count = reinterpret_cast<uint32_t *>(w.range + (size_t)group * w.splits);
+    w.listed = reinterpret_cast<int *>(w.count + bins);
     for (w.row0 = 0; w.row0 < n_rows; w.row0 += group) {
         const int rows = std::min(group, n_rows - w.row0);
         const dim3 grid((unsigned)w.splits, (unsigned)rows);
-        rt::sample_range_kernel<<<grid, 256, 0, ctx->stream>>>(a, w);
-        rt::sample_histogram_kernel<<<grid, 256, 0, ctx->stream>>>(a, w);
-        rt::sample_finish_kernel<<<dim3((unsigned)rows), rt::kFinishThreads, 0, ctx->stream>>>(a, w);
+        rt::sample_range_kernel<<<grid, rt::kThreads, 0, ctx->stream>>>(a, w);
+        rt::sample_histogram_kernel<<<grid, rt::kCountThreads, 0, ctx->stream>>>(a, w);
+        rt::sample_collect_kernel<<<dim3((unsigned)w.parts, (unsigned)rows), rt::kThreads, 0, ctx->stream>>>(a, w);
+        rt::sample_finish_kernel<<<dim3((unsigned)rows), rt::kThreads, 0, ctx->stream>>>(a, w);
     }
     RT_TRY_HIP(ctx, hipGetLastError());
     return RT_HIP_OK;
