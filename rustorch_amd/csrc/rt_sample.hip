@@ -47,14 +47,26 @@ __device__ __forceinline__ unsigned long long fixed_weight(float x, float top, d
     return (unsigned long long)rint(ldexp(weight_of(x, top, temperature), frac_bits));
 }
 
-__device__ __forceinline__ unsigned long long wave_sum_u64(unsigned long long v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)v, o), hi = (uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), o);
-        v += ((unsigned long long)hi << 32) | lo;
-    }
-    return v;
+// Running sum over the lanes of a wave, this one's included: shifts inside the rows of 16 lanes, then the rows' ends passed on
+// (one vector instruction a step; a shuffle through LDS takes ten times as long, and these sums wait for one another).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long dpp_add_u64(unsigned long long v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+    return v + (((unsigned long long)hi << 32) | lo);
 }
+__device__ __forceinline__ unsigned long long wave_scan_u64(unsigned long long v) {
+    v = dpp_add_u64<0x111, 0xf>(v);          // row_shr:1, 2, 4, 8
+    v = dpp_add_u64<0x112, 0xf>(v);
+    v = dpp_add_u64<0x114, 0xf>(v);
+    v = dpp_add_u64<0x118, 0xf>(v);
+    v = dpp_add_u64<0x142, 0xa>(v);          // row_bcast:15 into rows 1 and 3
+    return dpp_add_u64<0x143, 0xc>(v);       // row_bcast:31 into rows 2 and 3
+}
+__device__ __forceinline__ unsigned long long lane_u64(unsigned long long v, int l) {
+    return ((unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
+}
+__device__ __forceinline__ unsigned long long wave_sum_u64(unsigned long long v) { return lane_u64(wave_scan_u64(v), 63); }
 // Every thread of the workgroup gets the sum; red holds one value per wave.
 __device__ __forceinline__ unsigned long long block_sum_u64(unsigned long long v, unsigned long long *red) {
     v = wave_sum_u64(v);
@@ -68,14 +80,11 @@ __device__ __forceinline__ unsigned long long block_sum_u64(unsigned long long v
 }
 
 // ---- bins: a row's tokens by their distance d = M - l below the largest logit, up to the distance R beyond which the weight
-// rounds to zero (or the smallest finite logit, if that is nearer): the bin's number is floor(d * (kBins - 1) / R), which is
-// monotone in d.  The weight of a token is the weight at the middle of its kTable-th part of the reach, from a table, times
-// exp(-r), |r| <= 0.016, by its series to the sixth power (the next term is below 2^-54): a dozen 64-bit operations where exp()
-// takes four times as many.  The middle is the same rounded number in the table and in r, and so the product is as exact as
-// exp() itself.
-// 4096 bins hold at most a few dozen tokens each where the cuts of real rows fall; 1024 held hundreds, whose ranking (every one
-// against every other) took most of the time.
-constexpr int kBins = 4096, kTable = 1024, kThreads = 256, kCountThreads = 512, kListMost = 2048, kPart = 4096;
+// rounds to zero (or the smallest finite logit, if that is nearer).  The bin's number is d * (kBins - 1) / R in f32: only its
+// being monotone in d matters, and that the last bin ends past R.
+// 4096 bins hold at most a hundred tokens each where the cuts of real rows fall; 1024 held several hundred, whose ranking (every
+// one against every other) took most of the time.
+constexpr int kBins = 4096, kThreads = 256, kCountThreads = 1024, kCoarse = kBins / 64, kListMost = 2048, kPart = 4096;
 
 struct RowRange { float top, low; int arg, pad; };        // of one split of a row: largest logit, smallest finite one, index of the largest
 // What the histogram says of a row's cuts.
@@ -93,55 +102,57 @@ struct SampleWork {
     RowRange *range;                                       // [row][split]
     unsigned long long *sum;                               // [row][kBins]
     uint32_t *count;                                       // [row][kBins]
+    unsigned long long *coarse_sum;                        // [row][64], the same of kBins / 64 bins at a time
+    uint32_t *coarse_count;
     RowBorders *borders;                                   // [row]
     int *listed;                                           // [row]: tokens listed
     unsigned long long *list;                              // [row][kListMost]: their keys
     unsigned long long *part_sum;                          // [row][part]: weight that stays whole, of kPart tokens each
-    int row0, splits, per_split, parts;                    // this launch's first row
+    int row0, splits, per_split, per_count, parts;                    // this launch's first row
 };
 
 struct RowBins {
-    double top, scale, inv_t;
-    double width;                 // of a table entry
-    float topf;
+    double top, rate;             // rate = log2(e) / T
+    float topf, half_top, scale;
+    int frac_bits;
 };
 __device__ __forceinline__ RowBins row_bins(float top, float low, double T, int frac_bits) {
+    const double reach = (double)(frac_bits + 1) * 0.69314718055994531 * T, span = (double)top - (double)low, R = reach < span ? reach : span;
     RowBins b;
-    const double reach = (double)(frac_bits + 1) * 0.69314718055994531 * T, span = (double)top - (double)low;
-    const double R = reach < span ? reach : span;
-    b.topf = top;
     b.top = (double)top;
-    b.scale = R > 0.0 ? (double)(kBins - 1) / R : 0.0;
-    b.width = R / (double)(kBins - 1) * (double)(kBins / kTable);
-    b.inv_t = 1.0 / T;
+    b.rate = 1.4426950408889634 / T;
+    b.topf = top;
+    b.half_top = 0.5f * top;      // half of d always fits f32
+    b.scale = R > 0.0 ? fminf(2.0f * (float)(kBins - 1) / (float)(0.5 * R) * 0.5f, 1e37f) : 0.0f;
+    b.frac_bits = frac_bits;
     return b;
 }
-#pragma clang fp contract(off)
-__device__ __forceinline__ double entry_middle(const RowBins &b, int entry) { return ((double)entry + 0.5) * b.width; }
 __device__ __forceinline__ int bin_of(const RowBins &b, float x) {       // kBins: beyond the reach, NaN or infinite
-    const double at = (b.top - (double)x) * b.scale;
-    return at < (double)kBins ? (int)at : kBins;                         // false for NaN
+    const float at = (b.half_top - 0.5f * x) * b.scale;
+    return at < (float)kBins ? (int)at : kBins;                          // false for NaN
 }
-__device__ __forceinline__ void fill_table(const RowBins &b, int frac_bits, double *table) {
-    for (int i = threadIdx.x; i < kTable; i += blockDim.x) table[i] = ldexp(exp(-(entry_middle(b, i) * b.inv_t)), frac_bits);
-}
-// the weight times 2^frac_bits
-__device__ __forceinline__ double binned_weight(const RowBins &b, float x, int bin, const double *table, int frac_bits) {
-    if (x == b.topf) return ldexp(1.0, frac_bits);
-    const int entry = bin / (kBins / kTable);
-    const double r = ((b.top - (double)x) - entry_middle(b, entry)) * -b.inv_t;
-    double e = fma(r, 1.0 / 720.0, 1.0 / 120.0);
-    e = fma(e, r, 1.0 / 24.0);
-    e = fma(e, r, 1.0 / 6.0);
-    e = fma(e, r, 0.5);
-    e = fma(e, r, 1.0);
-    e = fma(e, r, 1.0);
-    return table[entry] * e;
+// exp((x - M) / T) * 2^frac_bits in 64 bits: 2^t with t split into a whole number and |f| <= 1/2, the latter by the series of the
+// exponential to the twelfth power (the next term is below 2^-52): eighteen operations, a third of what exp() takes.
+__device__ __forceinline__ double token_weight(const RowBins &b, float x) {
+    if (x == b.topf) return ldexp(1.0, b.frac_bits);
+    const double t = fmax(((double)x - b.top) * b.rate, -2000.0), n = rint(t), y = (t - n) * 0.69314718055994531;
+    double e = fma(y, 1.0 / 479001600.0, 1.0 / 39916800.0);
+    e = fma(e, y, 1.0 / 3628800.0);
+    e = fma(e, y, 1.0 / 362880.0);
+    e = fma(e, y, 1.0 / 40320.0);
+    e = fma(e, y, 1.0 / 5040.0);
+    e = fma(e, y, 1.0 / 720.0);
+    e = fma(e, y, 1.0 / 120.0);
+    e = fma(e, y, 1.0 / 24.0);
+    e = fma(e, y, 1.0 / 6.0);
+    e = fma(e, y, 0.5);
+    e = fma(e, y, 1.0);
+    e = fma(e, y, 1.0);
+    return ldexp(e, (int)n + b.frac_bits);
 }
 __device__ __forceinline__ unsigned long long whole(double w) {          // rounded to nearest, 0 <= w <= 2^51: the sum's last bits
     return __builtin_bit_cast(unsigned long long, w + 4503599627370496.0) - 0x4330000000000000ull;
 }
-#pragma clang fp contract(fast)
 
 // What a row asks for.
 struct RowAsks {
@@ -202,7 +213,13 @@ __global__ __launch_bounds__(kThreads) void sample_range_kernel(SampleArgs a, Sa
         }
         w.range[(size_t)row * w.splits + split] = RowRange{ top, low, arg, 0 };
     }
-    if (split == 0 && tid == 0) w.listed[row] = 0;
+    if (split == 0) {
+        if (tid == 0) w.listed[row] = 0;
+        if (tid < kCoarse) {
+            w.coarse_sum[(size_t)row * kCoarse + tid] = 0;
+            w.coarse_count[(size_t)row * kCoarse + tid] = 0;
+        }
+    }
     const int share = (kBins + w.splits - 1) / w.splits, b1 = min(kBins, (split + 1) * share);
     for (int b = split * share + tid; b < b1; b += 256) {
         w.sum[(size_t)row * kBins + b] = 0;
@@ -228,7 +245,6 @@ __device__ __forceinline__ RowRange row_range(const SampleWork &w, int row) {
 }
 
 __global__ __launch_bounds__(kCountThreads) void sample_histogram_kernel(SampleArgs a, SampleWork w) {
-    __shared__ double table[kTable];
     __shared__ unsigned long long sum[kBins];
     __shared__ uint32_t count[kBins];
     const int tid = threadIdx.x, split = blockIdx.x, row = blockIdx.y, r = w.row0 + row;
@@ -239,13 +255,12 @@ __global__ __launch_bounds__(kCountThreads) void sample_histogram_kernel(SampleA
     if (g.top == -INFINITY || g.top == INFINITY) return;                  // without weights
     const bool weighs = q.p > 0.f;                                        // top-k alone counts
     const RowBins b = row_bins(g.top, g.low, q.T, a.frac_bits);
-    if (weighs) fill_table(b, a.frac_bits, table);
     for (int i = tid; i < kBins; i += kCountThreads) {
         sum[i] = 0;
         count[i] = 0;
     }
     __syncthreads();
-    const int i0 = split * w.per_split, i1 = min(a.vocab, i0 + w.per_split);
+    const int i0 = split * w.per_count, i1 = min(a.vocab, i0 + w.per_count);
     for (int i = i0 + tid; i < i1; i += 8 * kCountThreads) {
         float v[8];
         load_steps(x, i, kCountThreads, i1, v);
@@ -253,17 +268,27 @@ __global__ __launch_bounds__(kCountThreads) void sample_histogram_kernel(SampleA
         for (int j = 0; j < 8; j++) {
             const int bin = bin_of(b, v[j]);
             if (bin < kBins) {
-                if (weighs) __hip_atomic_fetch_add(&sum[bin], whole(binned_weight(b, v[j], bin, table, a.frac_bits)), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                if (weighs) __hip_atomic_fetch_add(&sum[bin], whole(token_weight(b, v[j])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                 __hip_atomic_fetch_add(&count[bin], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             }
         }
     }
     __syncthreads();
-    for (int i = tid; i < kBins; i += kCountThreads)
-        if (count[i]) {
-            if (weighs) __hip_atomic_fetch_add(&w.sum[(size_t)row * kBins + i], sum[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            __hip_atomic_fetch_add(&w.count[(size_t)row * kBins + i], count[i], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    for (int i = tid; i < kBins; i += kCountThreads) {      // a wave has the 64 bins of one coarse bin
+        const uint32_t n = count[i];
+        const unsigned long long s = weighs ? sum[i] : 0;
+        const uint32_t n64 = (uint32_t)wave_sum_u64(n);
+        if (n64 == 0) continue;
+        const unsigned long long s64 = weighs ? wave_sum_u64(s) : 0;
+        if (n) {
+            __hip_atomic_fetch_add(&w.count[(size_t)row * kBins + i], n, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (weighs) __hip_atomic_fetch_add(&w.sum[(size_t)row * kBins + i], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         }
+        if ((tid & 63) == 0) {
+            __hip_atomic_fetch_add(&w.coarse_count[(size_t)row * kCoarse + i / 64], n64, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (weighs) __hip_atomic_fetch_add(&w.coarse_sum[(size_t)row * kCoarse + i / 64], s64, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        }
+    }
 }
 
 // A token's place in the order: ascending keys are descending logits, ascending indexes among equals.
@@ -272,12 +297,7 @@ __device__ __forceinline__ unsigned long long rank_key(float x, int i) { return 
 // Exclusive running sum over the workgroup's threads; red holds one value per wave, total the sum of all.
 __device__ __forceinline__ unsigned long long block_scan_u64(unsigned long long v, unsigned long long *red, unsigned long long &total) {
     const int lane = (int)(threadIdx.x & 63), wave = (int)(threadIdx.x >> 6);
-    unsigned long long s = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)s, o), hi = (uint32_t)__shfl_up((int)(uint32_t)(s >> 32), o);
-        if (lane >= o) s += ((unsigned long long)hi << 32) | lo;
-    }
+    const unsigned long long s = wave_scan_u64(v);
     __syncthreads();
     if (lane == 63) red[wave] = s;
     __syncthreads();
@@ -290,65 +310,59 @@ __device__ __forceinline__ unsigned long long block_scan_u64(unsigned long long 
     return before + s - v;
 }
 
-// The cuts' bins, from the row's histogram; the whole workgroup calls this and gets the answer in `out` (LDS).
-__device__ void find_borders(const SampleWork &w, int row, const RowAsks &q, unsigned long long *red, RowBorders &out) {
-    constexpr int kOwn = kBins / kThreads;
-    const int tid = threadIdx.x;
-    unsigned long long sum[kOwn], sums = 0, counts = 0, all_weight, all_tokens;
-    uint32_t count[kOwn];
-#pragma unroll
-    for (int j = 0; j < kOwn; j++) {
-        sum[j] = w.sum[(size_t)row * kBins + tid * kOwn + j];
-        count[j] = w.count[(size_t)row * kBins + tid * kOwn + j];
-    }
-#pragma unroll
-    for (int j = 0; j < kOwn; j++) {
-        sums += sum[j];
-        counts += count[j];
-    }
-    const unsigned long long n0 = block_scan_u64(counts, red, all_tokens), s0 = block_scan_u64(sums, red, all_weight);
-    const unsigned long long k = q.k > 0 && (unsigned long long)q.k < all_tokens ? (unsigned long long)q.k : 0;
-    if (tid == 0) out = RowBorders{ all_weight, all_weight, all_weight, 0, 0, k, 0, kBins, 0, -1, kBins };
-    __syncthreads();
-    if (k) {
-        unsigned long long n = n0, s = s0;
-#pragma unroll
-        for (int j = 0; j < kOwn; j++) {
-            if (n < k && k <= n + count[j]) {
-                out.k_bin = tid * kOwn + j;
-                out.k_weight_above = s;
-                out.k_weight_with = s + sum[j];
-                out.k_above = n;
-                out.k_in = count[j];
-            }
-            n += count[j];
-            s += sum[j];
+// The bin in which the running weight (or count) of a row's histogram reaches a goal: `reaches(before, with)` says whether a piece
+// is that one.  One wave: the coarse bins, then the 64 bins of the one found.  -1: none.
+template <class V, class F>
+__device__ __forceinline__ int find_bin(const V *fine, unsigned long long coarse, F reaches, unsigned long long &before, unsigned long long &in) {
+    const int lane = (int)(threadIdx.x & 63);
+    const unsigned long long upto = wave_scan_u64(coarse), group = __ballot(reaches(upto - coarse, upto));
+    if (!group) return -1;
+    const int c = __builtin_amdgcn_readfirstlane(__ffsll(group) - 1);
+    const unsigned long long base = lane_u64(upto - coarse, c), its = fine[c * 64 + lane], run = base + wave_scan_u64(its);
+    const unsigned long long bin = __ballot(reaches(run - its, run));
+    const int l = __builtin_amdgcn_readfirstlane(bin ? __ffsll(bin) - 1 : 63);
+    before = lane_u64(run - its, l);
+    in = lane_u64(its, l);
+    return c * 64 + l;
+}
+
+// The cuts' bins, from the row's histogram.  One wave calls this.
+__device__ RowBorders find_borders(const SampleWork &w, int row, const RowAsks &q) {
+    const int lane = (int)(threadIdx.x & 63);
+    const unsigned long long *sum = w.sum + (size_t)row * kBins;
+    const uint32_t *count = w.count + (size_t)row * kBins;
+    const unsigned long long coarse_sum = q.p > 0.f ? w.coarse_sum[(size_t)row * kCoarse + lane] : 0, coarse_count = w.coarse_count[(size_t)row * kCoarse + lane];
+    const unsigned long long all = wave_sum_u64(coarse_sum), tokens = wave_sum_u64(coarse_count);
+    RowBorders o{ all, all, all, 0, 0, q.k > 0 && (unsigned long long)q.k < tokens ? (unsigned long long)q.k : 0, 0, kBins, 0, -1, kBins };
+    unsigned long long in = 0;
+    if (o.k) {
+        const unsigned long long k = o.k;
+        o.k_bin = find_bin(count, coarse_count, [k](unsigned long long from, unsigned long long to) { return from < k && k <= to; }, o.k_above, o.k_in);
+        if (q.p > 0.f) {
+            const int c = o.k_bin / 64, l = o.k_bin % 64;
+            const unsigned long long base = lane_u64(wave_scan_u64(coarse_sum) - coarse_sum, c), its = sum[c * 64 + lane], run = base + wave_scan_u64(its);
+            o.k_weight_above = lane_u64(run - its, l);
+            o.k_weight_with = lane_u64(run, l);
         }
-        __syncthreads();
     }
+    o.keep_below = o.k_bin;
     if (q.p > 0.f) {
-        // the weight of the top k lies between that of the bins above its last one and that with it
-        const double lo = (double)q.p * (double)out.k_weight_above, hi = (double)q.p * (double)out.k_weight_with;
-        unsigned long long s = s0;
-#pragma unroll
-        for (int j = 0; j < kOwn; j++) {
-            const double from = (double)s, to = (double)(s + sum[j]);
-            if (sum[j] && from < lo && lo <= to) {
-                out.p_first = tid * kOwn + j;               // stays 0 where nothing lies above the bin of top-k
-                out.above_list = s;
-            }
-            if (sum[j] && from < hi && hi <= to) out.p_last = tid * kOwn + j;
-            s += sum[j];
+        // the weight of the top k lies between that of the bins above its last one and that with it; nothing above: from bin 0 on
+        const double lo = (double)q.p * (double)o.k_weight_above, hi = (double)q.p * (double)o.k_weight_with;
+        unsigned long long unused;
+        if (lo > 0.0) {
+            const int first = find_bin(sum, coarse_sum, [lo](unsigned long long from, unsigned long long to) { return (double)from < lo && lo <= (double)to; }, o.above_list, in);
+            o.p_first = max(first, 0);
         }
+        o.p_last = lo == hi ? o.p_first
+                            : find_bin(sum, coarse_sum, [hi](unsigned long long from, unsigned long long to) { return (double)from < hi && hi <= (double)to; }, unused, in);
+        o.keep_below = o.p_first;
     }
-    __syncthreads();
-    if (tid == 0) out.keep_below = q.p > 0.f ? out.p_first : out.k_bin;
-    __syncthreads();
+    return o;
 }
 
 // One workgroup per kPart tokens of a row: lists the tokens of the cuts' bins and sums the weights of the tokens above them.
 __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a, SampleWork w) {
-    __shared__ double table[kTable];
     __shared__ unsigned long long found[kListMost], red[kThreads / 64];
     __shared__ RowBorders borders;
     __shared__ int n_found, place;
@@ -359,14 +373,14 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a, 
     const RowRange g = row_range(w, row);
     if (g.top == -INFINITY || g.top == INFINITY) return;
     const RowBins b = row_bins(g.top, g.low, q.T, a.frac_bits);
-    fill_table(b, a.frac_bits, table);
-    if (tid == 0) n_found = 0;
-    if (q.k > 0 || q.p > 0.f) {
-        find_borders(w, row, q, red, borders);
-    } else {
-        if (tid == 0) borders = RowBorders{ 0, 0, 0, 0, 0, 0, 0, kBins, 0, -1, kBins };
-        __syncthreads();
+    if (tid < 64) {
+        const RowBorders o = q.k > 0 || q.p > 0.f ? find_borders(w, row, q) : RowBorders{ 0, 0, 0, 0, 0, 0, 0, kBins, 0, -1, kBins };
+        if (tid == 0) {
+            borders = o;
+            n_found = 0;
+        }
     }
+    __syncthreads();
     if (part == 0 && tid == 0) w.borders[row] = borders;
     const int k_bin = borders.k_bin, p_first = borders.p_first, p_last = borders.p_last, keep_below = borders.keep_below;
     const double min_w = ldexp(q.min_w, a.frac_bits);
@@ -380,7 +394,7 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a, 
             const int bin = bin_of(b, v[j]);
             if (bin >= kBins) continue;
             if (bin < keep_below) {
-                const double f = binned_weight(b, v[j], bin, table, a.frac_bits);
+                const double f = token_weight(b, v[j]);
                 if (f >= min_w) mine += whole(f);
             } else if (bin == k_bin || (bin >= p_first && bin <= p_last)) {
                 const int at = __hip_atomic_fetch_add(&n_found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
@@ -506,7 +520,6 @@ __device__ void sample_by_bisection(const SampleArgs &a, int r, const RowAsks &q
 
 __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, SampleWork w) {
     constexpr int kMine = kListMost / kThreads, kOwn = kPart / kThreads;
-    __shared__ double table[kTable];
     __shared__ unsigned long long buf[kPart];               // the list's keys and weights; the weights of one part; bisection's scratch
     __shared__ unsigned long long red[kThreads / 64], shared64[2];
     __shared__ int chosen;
@@ -531,8 +544,6 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, S
     const RowBins b = row_bins(g.top, g.low, q.T, a.frac_bits);
     const RowBorders c = w.borders[row];
     const double min_w = ldexp(q.min_w, a.frac_bits);
-    fill_table(b, a.frac_bits, table);
-    __syncthreads();
 
     // ---- the last key that stays
     unsigned long long cut = ~0ull;
@@ -548,7 +559,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, S
             if (i < n_list) {
                 key[m] = w.list[(size_t)row * kListMost + i];
                 const float v = order_logit(~(uint32_t)(key[m] >> 32));
-                own[m] = whole(binned_weight(b, v, bin_of(b, v), table, a.frac_bits));
+                own[m] = whole(token_weight(b, v));
                 list[i] = key[m];
                 list_weight[i] = own[m];
             }
@@ -556,13 +567,23 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, S
         __syncthreads();
         // every listed token's number and weight of listed tokens before it.  The listed bins are top-p's, one after the other, and
         // top-k's, which is the last of them or comes behind them.
-        for (int j = 0; j < n_list; j++) {
-            const unsigned long long other = list[j], its = list_weight[j];
+        // (eight at a time: the reads of LDS go out together)
+        for (int j0 = 0; j0 < n_list; j0 += 8) {
+            unsigned long long other[8], its[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                other[j] = j0 + j < n_list ? list[j0 + j] : ~0ull;
+                its[j] = list_weight[j0 + j];
+            }
 #pragma unroll
             for (int m = 0; m < kMine; m++)
-                if (m * kThreads < n_list && other < key[m]) {
-                    rank[m]++;
-                    weight_before[m] += its;
+                if (m * kThreads < n_list) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (other[j] < key[m]) {
+                            rank[m]++;
+                            weight_before[m] += its[j];
+                        }
                 }
         }
         double goal = (double)q.p * (double)c.all;
@@ -603,7 +624,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, S
         for (int m = 0; m < kMine; m++)
             if (tid + m * kThreads < n_list && key[m] <= cut) {
                 const float v = order_logit(~(uint32_t)(key[m] >> 32));
-                if (binned_weight(b, v, bin_of(b, v), table, a.frac_bits) >= min_w)
+                if (token_weight(b, v) >= min_w)
                     __hip_atomic_fetch_add(&buf[(uint32_t)key[m] / kPart], own[m], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             }
         __syncthreads();
@@ -627,7 +648,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, S
         const int i = i0 + j * kThreads + tid, bin = bin_of(b, v[j]);
         unsigned long long weight = 0;
         if (bin < kBins && rank_key(v[j], i) <= cut) {
-            const double f = binned_weight(b, v[j], bin, table, a.frac_bits);
+            const double f = token_weight(b, v[j]);
             if (f >= min_w) weight = whole(f);
         }
         buf[j * kThreads + tid] = weight;
@@ -643,7 +664,7 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, S
             if (weight && goal < at + weight) {
                 const int i = i0 + tid * kOwn + j;
                 a.out_token[r] = i;
-                if (a.out_prob) a.out_prob[r] = (float)(binned_weight(b, x[i], bin_of(b, x[i]), table, a.frac_bits) / (double)total);
+                if (a.out_prob) a.out_prob[r] = (float)(token_weight(b, x[i]) / (double)total);
                 break;
             }
             at += weight;
@@ -671,28 +692,34 @@ int rt_hip_sample_dev(rt_hip_ctx *ctx, const float *logits, size_t ld, int n_row
     int bits = 0;
     while ((1 << bits) < vocab) bits++;
     rt::SampleArgs a{ logits, ld, n_rows, vocab, bits < 11 ? 51 : 62 - bits, u, temperature, top_p, min_p, top_k, out_token, out_prob };
-    // a row is split so that about a thousand workgroups share the first two launches, 2048 tokens at least in each; rows go in
-    // groups whose histograms stay below 64 MB
+    // A row is split so that about a thousand workgroups look for the ranges (2048 tokens at least in each) and as many as there are
+    // compute units count (4096 tokens at least): every one of the latter adds up to 4096 bins to the row's histogram.  77 rows
+    // of 131071: 71 us with 256 workgroups, 73 with 512, 81 with 1024.  Rows go in groups whose histograms stay below 64 MB.
     const int group = std::min(n_rows, 1024);
     rt::SampleWork w;
     w.splits = std::max(1, std::min(1024 / group, (vocab + 2047) / 2048));
+    const int count_splits = std::max(1, std::min(256 / group, (vocab + 4095) / 4096));
     w.per_split = (vocab + w.splits - 1) / w.splits;
+    w.per_count = (vocab + count_splits - 1) / count_splits;
     w.parts = (vocab + rt::kPart - 1) / rt::kPart;
-    const size_t bins = (size_t)group * rt::kBins, list = (size_t)group * rt::kListMost, parts = (size_t)group * w.parts;
-    int rc = ensure_scratch(ctx, (bins + list + parts) * 8 + group * sizeof(rt::RowBorders) + (size_t)group * w.splits * sizeof(rt::RowRange) + bins * 4 + (size_t)group * 4);
+    const size_t coarse = (size_t)group * rt::kCoarse, bins = (size_t)group * rt::kBins, list = (size_t)group * rt::kListMost, parts = (size_t)group * w.parts;
+    int rc = ensure_scratch(ctx, (bins + list + parts + coarse) * 8 + group * sizeof(rt::RowBorders) + (size_t)group * w.splits * sizeof(rt::RowRange) +
+                                 (bins + coarse + group) * 4);
     if (rc) return rc;
     w.sum = static_cast<unsigned long long *>(ctx->scratch);
     w.list = w.sum + bins;
     w.part_sum = w.list + list;
-    w.borders = reinterpret_cast<rt::RowBorders *>(w.part_sum + parts);
+    w.coarse_sum = w.part_sum + parts;
+    w.borders = reinterpret_cast<rt::RowBorders *>(w.coarse_sum + coarse);
     w.range = reinterpret_cast<rt::RowRange *>(w.borders + group);
     w.count = reinterpret_cast<uint32_t *>(w.range + (size_t)group * w.splits);
-    w.listed = reinterpret_cast<int *>(w.count + bins);
+    w.coarse_count = w.count + bins;
+    w.listed = reinterpret_cast<int *>(w.coarse_count + coarse);
     for (w.row0 = 0; w.row0 < n_rows; w.row0 += group) {
         const int rows = std::min(group, n_rows - w.row0);
         const dim3 grid((unsigned)w.splits, (unsigned)rows);
         rt::sample_range_kernel<<<grid, rt::kThreads, 0, ctx->stream>>>(a, w);
-        rt::sample_histogram_kernel<<<grid, rt::kCountThreads, 0, ctx->stream>>>(a, w);
+        rt::sample_histogram_kernel<<<dim3((unsigned)count_splits, (unsigned)rows), rt::kCountThreads, 0, ctx->stream>>>(a, w);
         rt::sample_collect_kernel<<<dim3((unsigned)w.parts, (unsigned)rows), rt::kThreads, 0, ctx->stream>>>(a, w);
         rt::sample_finish_kernel<<<dim3((unsigned)rows), rt::kThreads, 0, ctx->stream>>>(a, w);
     }

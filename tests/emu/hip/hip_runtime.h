@@ -207,6 +207,7 @@ inline int emu_update_dpp(int old, int src, int ctrl, int row_mask, int /*bank_m
     if (ctrl < 0x100) from = (l & ~3) + ((ctrl >> (2 * (l & 3))) & 3);   // quad_perm
     else if (ctrl == 0x141) from = (l & ~7) + (7 - (l & 7));               // row_half_mirror
     else if (ctrl == 0x140) from = (l & ~15) + (15 - (l & 15));            // row_mirror
+    else if (ctrl > 0x110 && ctrl < 0x120) { from = l - (ctrl & 15); if ((l & 15) < (ctrl & 15)) { from = l; write = false; } }   // row_shr
     else if (ctrl == 0x142) { from = (l & ~15) - 1; if (l < 16) { from = l; write = false; } }   // row_bcast:15
     else if (ctrl == 0x143) { from = 31; if (l < 32) { from = l; write = false; } }              // row_bcast:31
     int got = (int)emu::wave_exchange((uint32_t)src, from);
