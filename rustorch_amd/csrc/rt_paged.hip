@@ -273,8 +273,10 @@ int rt_hip_paged_attn_prefill_dev(rt_hip_ctx *ctx, const rt_hip_paged_kv *kv, co
     int rc = batch_check(ctx, who, kv, block_table, max_blocks, kv_len, n_seq);
     if (rc) return rc;
     RT_REQUIRE(ctx, q && out && cu_new, RT_HIP_ERR_INVALID_ARG, "%s: NULL argument", who);
-    RT_REQUIRE(ctx, n_tok >= 0 && n_tok <= 65535, RT_HIP_ERR_SHAPE, "%s: n_tok=%d outside 0..65535", who, n_tok);
+    RT_REQUIRE(ctx, n_tok >= 0, RT_HIP_ERR_SHAPE, "%s: n_tok=%d", who, n_tok);
     if ((rc = heads_check(ctx, who, kv, n_heads))) return rc;
+    RT_REQUIRE(ctx, (long long)n_tok * (n_heads / kv->n_kv_heads) / 64 + n_seq <= 65535, RT_HIP_ERR_SHAPE, "%s: %d tokens of %d heads per key / value head are beyond one grid",
+               who, n_tok, n_heads / kv->n_kv_heads);
     const size_t row = (size_t)n_heads * kv->head_dim;
     if ((rc = rows_check(ctx, who, "q", q, q_ld, row)) || (rc = rows_check(ctx, who, "out", out, out_ld, row))) return rc;
     if (n_tok == 0) return RT_HIP_OK;

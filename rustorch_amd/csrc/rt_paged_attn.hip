@@ -386,26 +386,56 @@ hipError_t launch_paged_decode(hipStream_t s, const PagedView &p, int head_dim, 
 }
 
 namespace {
-// One wave per (row, query head): the positions one after the other with a running maximum and sum.
+
+// --------------------------------------------------------------------------------------------- several queries per sequence
+// Bound by the matrix cores.  The rows of one kv head of one sequence -- its new tokens times the query heads that share the kv
+// head -- are packed one after the other; a wave has 32 of them, a workgroup 32 W, and the workgroup's keys and values go through
+// LDS once for all of them.  Flash style, tiles of 32 positions:
+//   S^T[key][row]  = K . (Qhi + Qlo)^T    v_mfma_f32_32x32x16_f16, the f32 side in two halves (value = hi + lo after a power-of-two
+//                                         scaling): f32 accuracy for twice the products.  A lane's 16 scores belong to one row.
+//   O^T[dim][row]  = V^T . (Phi + Plo)^T  a lane's 16 probabilities are, as they stand, the second operand; the first wants four
+//                                         consecutive keys of one dim per register pair, which ds_read_b64_tr_b16 reads from the
+//                                         row-major tile.
+// Chunks of 16 bytes are swizzled inside their rows so that both kinds of reads meet all banks.  The next tile waits in registers
+// while the current one is used, the one behind it is requested then: one barrier per tile.
+// The grid runs kv heads first: neighbouring workgroups land on different XCDs, so an XCD sees few kv heads and keeps their keys and
+// values in its L2; later rows, which have more keys, go first.
+// An infinite or NaN value at a position that some of a tile's rows do not see would enter their sums as 0 * inf.  Tiles that
+// reach beyond a row are looked through for such values; a workgroup that meets one does its rows again, one at a time.
+constexpr int kPrefillKeys = 32;
+
+struct PrefillArgs {
+    PagedView p;
+    const float *q;
+    float *out;
+    size_t q_ld, out_ld;
+    int n_tok, n_heads, group;
+};
+
+// ds_read_b64_tr_b16: in each 16 lanes, lane i gets the i-th column of the 4 x 16 matrix whose row r is the 8 bytes each of lanes 4 r .. 4 r + 3
+typedef short short4v __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) short4v lds_short4v;
+typedef _Float16 half4v __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ half4v read_transposed(const uint16_t *p) { return __builtin_bit_cast(half4v, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4v *)p)); }
+
+typedef float float16v __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// One row of one query head by one wave, the positions one after the other: nothing that is not seen is touched.
 template <int HD>
-__global__ __launch_bounds__(64) void paged_attn_kernel(PagedView p, const float *q, size_t q_ld, int n_heads, float *out, size_t out_ld) {
+__device__ void attend_row(const PagedView &p, const float *q, float *out, int seq, int kvh, int n) {
     constexpr int E = HD / 64;               // elements of the head a lane holds
-    const int h = blockIdx.x, t = blockIdx.y, lane = threadIdx.x;
-    int seq;
-    long long pos;
-    if (!row_place(p, t, seq, pos)) return;
-    const int kvh = h / (n_heads / p.n_kv);
-    const long long width = (long long)p.max_blocks << p.page_shift, n = min(pos + 1, width);
+    const int lane = (int)(threadIdx.x & 63);
     const float scale = 1.0f / sqrtf((float)HD);
     float qv[E], acc[E], m = -INFINITY, l = 0.f;
     for (int e = 0; e < E; e++) {
-        qv[e] = q[(size_t)t * q_ld + (size_t)h * HD + E * lane + e] * scale;
+        qv[e] = q[E * lane + e] * scale;
         acc[e] = 0.f;
     }
-    for (long long j = 0; j < n; j++) {
-        const int page = p.table[(size_t)seq * p.max_blocks + (size_t)(j >> p.page_shift)];
+    for (int j = 0; j < n; j++) {
+        const int page = p.table[(size_t)seq * p.max_blocks + (j >> p.page_shift)];
         if (page < 0 || page >= p.n_pages) continue;
-        const size_t at = ((((size_t)page * p.n_kv + kvh) << p.page_shift) + (size_t)(j & ((1ll << p.page_shift) - 1))) * HD + E * lane;
+        const size_t at = ((((size_t)page * p.n_kv + kvh) << p.page_shift) + (size_t)(j & ((1 << p.page_shift) - 1))) * HD + E * lane;
         float s = 0.f;
         for (int e = 0; e < E; e++) s += qv[e] * h2f(p.k[at + e]);
         s = wave_sum(s);
@@ -415,15 +445,247 @@ __global__ __launch_bounds__(64) void paged_attn_kernel(PagedView p, const float
         for (int e = 0; e < E; e++) acc[e] = acc[e] * keep + w * h2f(p.v[at + e]);
         m = m_new;
     }
-    for (int e = 0; e < E; e++) out[(size_t)t * out_ld + (size_t)h * HD + E * lane + e] = l > 0.f ? acc[e] / l : (l == 0.f ? 0.f : l);
+    for (int e = 0; e < E; e++) out[E * lane + e] = l == 0.f ? 0.f : acc[e] / l;
+}
+
+template <int HD, int W>
+__global__ __launch_bounds__(64 * W, 2) void paged_prefill_kernel(PrefillArgs a) {
+    constexpr int KK = HD / 16, DB = HD / 32, CPR = HD / 8, TQ = 32 * W, KT = kPrefillKeys;
+    constexpr int ROWS_AT_ONCE = 64 * W / CPR, NL = KT / ROWS_AT_ONCE;     // rows of a tile that the workgroup's threads load at once, and how often
+    static_assert(NL >= 1 && (16 % ROWS_AT_ONCE == 0 || ROWS_AT_ONCE % 16 == 0), "a load covers whole groups of 16 positions or lies inside one");
+    __shared__ __align__(16) uint16_t ks[2][KT * HD], vs[2][KT * HD];
+    __shared__ int odd;                      // some value that not every row sees is not finite
+    const PagedView &p = a.p;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), j = lane & 31, hh = lane >> 5;
+    const int kvh = blockIdx.x, tile = (int)(gridDim.y - 1 - blockIdx.y);
+
+    // ---- which rows: sequence s has the tiles from floor(cu_new[s] * group / TQ) + s on
+    int seq = 0;
+    for (int s0 = 1; s0 < p.n_seq; s0 += 64) {
+        const int s = s0 + lane;
+        const unsigned long long begun = __ballot(s < p.n_seq && (long long)p.cu_new[s] * a.group / TQ + s <= tile);
+        seq += __popcll(begun);
+        if (begun != ~0ull) break;
+    }
+    const int t0 = p.cu_new[seq], t1 = p.cu_new[seq + 1];
+    if (t0 < 0 || t1 > a.n_tok || t1 <= t0) return;
+    const long long first_row = (tile - ((long long)t0 * a.group / TQ + seq)) * TQ;
+    const int n_rows = (int)min((long long)TQ, (long long)(t1 - t0) * a.group - first_row);
+    if (first_row < 0 || n_rows <= 0) return;
+    const int width = p.max_blocks << p.page_shift, new_tok = t1 - t0;
+    auto place = [&](int row, int &tok, int &head) -> int {       // of a row of the tile; returns the positions it sees
+        const long long r = first_row + row;
+        tok = (int)(r / a.group);
+        head = (int)(r - (long long)tok * a.group);
+        return (int)max(0ll, min((long long)width, (long long)p.kv_len[seq] - new_tok + tok + 1));
+    };
+    int tok, head_in_group, least, most;
+    least = place(0, tok, head_in_group);                         // positions that the first row sees: every row sees them
+    most = place(n_rows - 1, tok, head_in_group);
+    const int seen = place(min(32 * wave + j, n_rows - 1), tok, head_in_group);
+    const int wave_most = [&] { int t, h; return 32 * wave < n_rows ? place(min(32 * wave + 31, n_rows - 1), t, h) : 0; }();
+    const float *qrow = a.q + (size_t)(t0 + tok) * a.q_ld + (size_t)(kvh * a.group + head_in_group) * HD;
+    float *orow = a.out + (size_t)(t0 + tok) * a.out_ld + (size_t)(kvh * a.group + head_in_group) * HD;
+    const bool has_row = 32 * wave + j < n_rows;
+    if (tid == 0) odd = 0;
+
+    // ---- the query fragments: lane (j, hh) holds elements 16 kk + 8 hh .. + 7 of its row
+    half8v qhi[KK], qlo[KK];
+    float sscale;
+    {
+        float amax = 0.f;
+        for (int kk = 0; kk < KK; kk++) {
+            const float4 x = *reinterpret_cast<const float4 *>(qrow + 16 * kk + 8 * hh), y = *reinterpret_cast<const float4 *>(qrow + 16 * kk + 8 * hh + 4);
+            amax = fmaxf(amax, fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))), fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)))));
+        }
+        amax = fmaxf(amax, __shfl_xor(amax, 32));
+        int ex = 0;
+        if (amax > 0.f) frexpf(amax, &ex);               // amax = f * 2^ex, f in [0.5, 1)
+        ex = max(ex, -100);
+        const float qscale = ldexpf(1.0f, 14 - ex);
+        sscale = ldexpf(1.0f, ex - 14) * (1.44269504088896341f / sqrtf((float)HD));       // scores in units of log2
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) {
+            const float4 x = *reinterpret_cast<const float4 *>(qrow + 16 * kk + 8 * hh), y = *reinterpret_cast<const float4 *>(qrow + 16 * kk + 8 * hh + 4);
+            const float f[8] = { x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w };
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float v = f[e] * qscale;
+                const _Float16 hi = (_Float16)v;
+                qhi[kk][e] = hi;
+                qlo[kk][e] = (_Float16)(v - (float)hi);
+            }
+        }
+    }
+
+    // ---- tiles: a thread brings chunk c of rows r0 + i * ROWS_AT_ONCE
+    const int tiles = (most + KT - 1) / KT, r0 = tid / CPR, c = tid % CPR;
+    u32x4 kreg[NL], vreg[NL];
+    int good = 0;                            // bit g: positions 16 g .. of the requested tile lie on a page of the pool
+    auto request = [&](int t) {
+        good = 0;
+        size_t base[KT / 16];
+#pragma unroll
+        for (int g = 0; g < KT / 16; g++) {
+            const int key = t * KT + 16 * g, pg = key >> p.page_shift;
+            const int id = pg < p.max_blocks ? p.table[(size_t)seq * p.max_blocks + pg] : -1;
+            const bool ok = id >= 0 && id < p.n_pages;
+            good |= ok ? 1 << g : 0;
+            base[g] = ((((size_t)(ok ? id : 0) * p.n_kv + kvh) << p.page_shift) + (size_t)(key & ((1 << p.page_shift) - 1))) * HD;
+        }
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int r = r0 + i * ROWS_AT_ONCE;
+            const size_t at = (r >= 16 ? base[1] : base[0]) + (size_t)(r & 15) * HD + 8 * c;
+            kreg[i] = *reinterpret_cast<const u32x4 *>(p.k + at);
+            vreg[i] = *reinterpret_cast<const u32x4 *>(p.v + at);
+        }
+    };
+    auto put = [&](int t, int buf, int ok) {             // the requested tile t goes to LDS; values that no row sees as zeros
+        const bool whole = (t + 1) * KT <= least && ok == (1 << (KT / 16)) - 1;
+        if (!whole) {
+            uint32_t found = 0;
+#pragma unroll
+            for (int i = 0; i < NL; i++) {
+                const int r = r0 + i * ROWS_AT_ONCE;
+                const bool is = t * KT + r < most && ((ok >> (r >> 4)) & 1);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    vreg[i][e] = is ? vreg[i][e] : 0u;
+                    found |= (uint32_t)((vreg[i][e] & 0x7C00u) == 0x7C00u) | (uint32_t)((vreg[i][e] & 0x7C000000u) == 0x7C000000u);
+                }
+            }
+            if (found) odd = 1;
+        }
+#pragma unroll
+        for (int i = 0; i < NL; i++) {
+            const int r = r0 + i * ROWS_AT_ONCE;
+            const int vc = HD == 128 ? c ^ (4 * (r & 3)) : c ^ (4 * ((r >> 1) & 1));
+            *reinterpret_cast<u32x4 *>(&ks[buf][r * HD + 8 * (c ^ (r & (CPR - 1)))]) = kreg[i];
+            *reinterpret_cast<u32x4 *>(&vs[buf][r * HD + 8 * vc]) = vreg[i];
+        }
+    };
+
+    float16v acc[DB];
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) acc[db][r] = 0.f;
+    float m_run = -INFINITY, l_run = 0.f;
+    int ok_now = 0, ok_next = 0;
+    if (tiles > 0) {
+        request(0);
+        ok_now = good;
+        __syncthreads();                                  // odd is cleared before anyone sets it
+        put(0, 0, ok_now);
+        request(min(1, tiles - 1));
+        ok_next = good;
+    }
+    __syncthreads();
+    // the value rows of the transposed reads: source lane s of a group of 16 reads 4 dims of row s / 4
+    const int s16 = lane & 15, vrow0 = 4 * hh + (s16 >> 2), vcol0 = 16 * ((lane >> 4) & 1) + 4 * (s16 & 3);
+    for (int t = 0; t < tiles; t++) {
+        const int buf = t & 1;
+        if (t * KT < wave_most) {
+            float16v s;
+#pragma unroll
+            for (int r = 0; r < 16; r++) s[r] = 0.f;
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) {
+                const half8v k = *reinterpret_cast<const half8v *>(&ks[buf][j * HD + 8 * ((2 * kk + hh) ^ (j & (CPR - 1)))]);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qhi[kk], s, 0, 0, 0);
+                s = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, qlo[kk], s, 0, 0, 0);
+            }
+            // register r is position 8 (r / 4) + 4 hh + r % 4 of the tile against the lane's row
+            if ((t + 1) * KT <= least && ok_now == (1 << (KT / 16)) - 1) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[r] *= sscale;
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; r++) {
+                    const int at = 8 * (r >> 2) + 4 * hh + (r & 3);
+                    s[r] = t * KT + at < seen && ((ok_now >> (at >> 4)) & 1) ? s[r] * sscale : -INFINITY;
+                }
+            }
+            float mt = m_run;
+#pragma unroll
+            for (int r = 0; r < 16; r++) mt = fmaxf(mt, s[r]);
+            mt = fmaxf(mt, __shfl_xor(mt, 32));
+            const float m_ref = mt == -INFINITY ? 0.f : mt;      // nothing seen yet
+            if (__ballot(mt > m_run)) {
+                const float alpha = __builtin_amdgcn_exp2f(m_run - m_ref);
+                l_run *= alpha;
+#pragma unroll
+                for (int db = 0; db < DB; db++)
+#pragma unroll
+                    for (int r = 0; r < 16; r++) acc[db][r] *= alpha;
+                m_run = mt;
+            }
+            half8v phi[2], plo[2];
+#pragma unroll
+            for (int r = 0; r < 16; r++) {
+                const float w = __builtin_amdgcn_exp2f(s[r] - m_ref);
+                l_run += w;
+                const float ws = w * 16384.0f;               // the lower half stays a normal number
+                const _Float16 hi = (_Float16)ws;
+                phi[r >> 3][r & 7] = hi;
+                plo[r >> 3][r & 7] = (_Float16)(ws - (float)hi);
+            }
+            // slot e of product mm stands for row 16 mm + 8 (e / 4) + 4 hh + e % 4 of the tile
+#pragma unroll
+            for (int db = 0; db < DB; db++)
+#pragma unroll
+                for (int mm = 0; mm < 2; mm++) {
+                    half8v av;
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const int row = 16 * mm + 8 * h + vrow0, col = 32 * db + vcol0, ch = col >> 3;
+                        const int vc = HD == 128 ? ch ^ (4 * (row & 3)) : ch ^ (4 * ((row >> 1) & 1));
+                        const half4v x = read_transposed(&vs[buf][row * HD + 8 * vc + (col & 7)]);
+#pragma unroll
+                        for (int e = 0; e < 4; e++) av[4 * h + e] = x[e];
+                    }
+                    acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, phi[mm], acc[db], 0, 0, 0);
+                    acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, plo[mm], acc[db], 0, 0, 0);
+                }
+        }
+        if (t + 1 < tiles) {
+            put(t + 1, buf ^ 1, ok_next);
+            ok_now = ok_next;
+            request(min(t + 2, tiles - 1));
+            ok_next = good;
+        }
+        __syncthreads();
+    }
+    if (odd) {
+        for (int row = wave; row < n_rows; row += W) {
+            int t, h;
+            const int n = place(row, t, h);
+            attend_row<HD>(p, a.q + (size_t)(t0 + t) * a.q_ld + (size_t)(kvh * a.group + h) * HD, a.out + (size_t)(t0 + t) * a.out_ld + (size_t)(kvh * a.group + h) * HD, seq,
+                           kvh, n);
+        }
+        return;
+    }
+    l_run += __shfl_xor(l_run, 32);
+    const float inv = l_run == 0.f ? 0.f : 1.0f / (l_run * 16384.0f);
+    if (!has_row) return;
+    // register r of block db is dim 32 db + 8 (r / 4) + 4 hh + r % 4
+#pragma unroll
+    for (int db = 0; db < DB; db++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            *reinterpret_cast<float4 *>(orow + 32 * db + 8 * g + 4 * hh) =
+                make_float4(acc[db][4 * g] * inv, acc[db][4 * g + 1] * inv, acc[db][4 * g + 2] * inv, acc[db][4 * g + 3] * inv);
 }
 
 }  // namespace
 
 hipError_t launch_paged_prefill(hipStream_t s, const PagedView &p, int head_dim, int n_tok, const float *q, size_t q_ld, int n_heads, float *out, size_t out_ld) {
-    const dim3 grid((unsigned)n_heads, (unsigned)n_tok);
-    if (head_dim == 128) paged_attn_kernel<128><<<grid, 64, 0, s>>>(p, q, q_ld, n_heads, out, out_ld);
-    else paged_attn_kernel<64><<<grid, 64, 0, s>>>(p, q, q_ld, n_heads, out, out_ld);
+    PrefillArgs a{ p, q, out, q_ld, out_ld, n_tok, n_heads, n_heads / p.n_kv };
+    constexpr int W = 4;
+    const dim3 grid((unsigned)p.n_kv, (unsigned)((long long)n_tok * a.group / (32 * W) + p.n_seq));
+    if (head_dim == 128) paged_prefill_kernel<128, W><<<grid, 64 * W, 0, s>>>(a);
+    else paged_prefill_kernel<64, W><<<grid, 64 * W, 0, s>>>(a);
     return hipGetLastError();
 }
 

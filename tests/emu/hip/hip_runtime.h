@@ -371,6 +371,20 @@ inline emu_f32x4 emu_mfma_f32_16x16x4f32(float a, float b, emu_f32x4 c) {
 #define __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, cbsz, abid, blgp) emu_mfma_f32_16x16x4f32(a, b, c)
 #define __builtin_amdgcn_exp2f(x) std::exp2((float)(x))
 
+// ds_read_b64_tr_b16: every lane names 8 bytes of LDS; in each 16 lanes, lane i gets halfword i % 4 of what lanes i / 4, 4 + i / 4,
+// 8 + i / 4, 12 + i / 4 named
+typedef short emu_i16x4 __attribute__((ext_vector_type(4)));
+inline emu_i16x4 emu_ds_read_tr16_b64(const void *p) {
+    emu_i16x4 mine;
+    memcpy(&mine, p, 8);
+    const emu_i16x4 *all = static_cast<const emu_i16x4 *>(emu::wave_gather(&mine, sizeof mine));
+    const int l = emu::lane_id(), i = l & 15;
+    emu_i16x4 r;
+    for (int e = 0; e < 4; e++) r[e] = all[(l & ~15) + 4 * e + i / 4][i % 4];
+    return r;
+}
+#define __builtin_amdgcn_ds_read_tr16_b64_v4i16(p) emu_ds_read_tr16_b64((const void *)(p))
+
 // v_mfma_f32_32x32x2f32: lane l holds A[l % 32][l / 32] and B[l / 32][l % 32]; D as for the other 32 x 32 shapes
 inline emu_f32x16 emu_mfma_f32_32x32x2f32(float a, float b, emu_f32x16 c) {
     struct { float a, b; } mine{ a, b };
