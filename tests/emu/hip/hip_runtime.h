@@ -371,6 +371,21 @@ inline emu_f32x4 emu_mfma_f32_16x16x4f32(float a, float b, emu_f32x4 c) {
 #define __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, cbsz, abid, blgp) emu_mfma_f32_16x16x4f32(a, b, c)
 #define __builtin_amdgcn_exp2f(x) std::exp2((float)(x))
 
+// v_cvt_pkrtz_f16_f32: two f32 cut to fp16 (towards zero)
+typedef _Float16 emu_f16x2 __attribute__((ext_vector_type(2)));
+inline _Float16 emu_cut_f16(float v) {
+    _Float16 h = (_Float16)v;
+    if (v == v && std::fabs((float)h) > std::fabs(v)) {          // rounded away from zero: one step back (an overflow becomes the largest)
+        uint16_t b;
+        memcpy(&b, &h, 2);
+        b--;
+        memcpy(&h, &b, 2);
+    }
+    return h;
+}
+inline emu_f16x2 emu_cvt_pkrtz(float a, float b) { return emu_f16x2{ emu_cut_f16(a), emu_cut_f16(b) }; }
+#define __builtin_amdgcn_cvt_pkrtz(a, b) emu_cvt_pkrtz(a, b)
+
 // ds_read_b64_tr_b16: every lane names 8 bytes of LDS; in each 16 lanes, lane i gets halfword i % 4 of what lanes i / 4, 4 + i / 4,
 // 8 + i / 4, 12 + i / 4 named
 typedef short emu_i16x4 __attribute__((ext_vector_type(4)));

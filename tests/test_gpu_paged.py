@@ -432,3 +432,29 @@ def test_paged_calls_refuse_what_they_cannot_do(ex):
     assert lib.rt_hip_paged_attn_decode_dev(ex.ctx, None, None, 0, None, 0, 0, None, 0, 0, None, 0) == 1
     assert lib.rt_hip_paged_attn_prefill_dev(ex.ctx, None, None, 0, None, None, 0, 0, None, 0, 0, None, 0) == 1
     ex.synchronize()
+
+
+def test_prefill_attention_of_more_sequences_than_a_wave_has_lanes(ex):
+    rng = np.random.default_rng(24)
+    new = [int(x) for x in rng.integers(0, 4, 70)]
+    b = ref.Batch(rng, [n + int(x) for n, x in zip(new, rng.integers(0, 20, 70))], 16, 1, 64, new)
+    check_prefill(ex, rng, b, 3)
+    check_decode(ex, rng, ref.Batch(rng, [int(x) for x in rng.integers(0, 400, 130)], 16, 1, 64), 1)
+
+
+@pytest.mark.parametrize("group", [1, 4])
+def test_prefill_attention_of_a_long_prompt(ex, group):
+    """As many rows as the launch for full devices is taken for; every 37th row is looked at."""
+    rng = np.random.default_rng(25)
+    n, n_kv, hd = 1600, 8 * 4 // group, 64
+    b = ref.Batch(rng, [n + 3], 64, n_kv, hd, [n])
+    d = OnDevice(ex, b)
+    q = rng.standard_normal((n, n_kv * group * hd)).astype(np.float32)
+    dout = ex.buffer(q.nbytes)
+    ex.paged_attn_prefill_dev(d.pool, d.seqs, ex.to_device(q), n, n_kv * group, dout)
+    got = dout.download(np.float32).reshape(q.shape)
+    for t in range(0, n, 37):
+        h = (t * 7) % (n_kv * group)
+        _, k, v = b.rows(0, h // group, 4 + t)
+        want, bound = ref.attention(q[t, h * hd:(h + 1) * hd].astype(np.float64), k, v, hd ** -0.5)
+        assert (np.abs(got[t, h * hd:(h + 1) * hd] - want) <= bound).all(), (t, h)
