@@ -67,6 +67,26 @@ __device__ __forceinline__ unsigned long long lane_u64(unsigned long long v, int
     return ((unsigned long long)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, l);
 }
 __device__ __forceinline__ unsigned long long wave_sum_u64(unsigned long long v) { return lane_u64(wave_scan_u64(v), 63); }
+// the wave's largest value, smallest value, by the same steps
+template <class F>
+__device__ __forceinline__ int wave_fold(int v, F f) {
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x111, 0xf, 0xf, false));
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x112, 0xf, 0xf, false));
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x114, 0xf, 0xf, false));
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x118, 0xf, 0xf, false));
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x142, 0xa, 0xf, false));
+    v = f(v, __builtin_amdgcn_update_dpp(v, v, 0x143, 0xc, 0xf, false));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+__device__ __forceinline__ float wave_top(float v) {
+    return __int_as_float(wave_fold(__float_as_int(v), [](int a, int b) { return __float_as_int(fmaxf(__int_as_float(a), __int_as_float(b))); }));
+}
+__device__ __forceinline__ float wave_low(float v) {
+    return __int_as_float(wave_fold(__float_as_int(v), [](int a, int b) { return __float_as_int(fminf(__int_as_float(a), __int_as_float(b))); }));
+}
+__device__ __forceinline__ int wave_low(int v) {
+    return wave_fold(v, [](int a, int b) { return min(a, b); });
+}
 // Every thread of the workgroup gets the sum; red holds one value per wave.
 __device__ __forceinline__ unsigned long long block_sum_u64(unsigned long long v, unsigned long long *red) {
     v = wave_sum_u64(v);
@@ -162,9 +182,13 @@ struct RowAsks {
     bool greedy;
 };
 __device__ __forceinline__ RowAsks row_asks(const SampleArgs &a, int r) {
-    const float t = a.temperature ? a.temperature[r] : 1.0f, p = a.top_p ? a.top_p[r] : 0.f, low = a.min_p ? a.min_p[r] : 0.f;
+    // one load each, none behind a branch, so that they go out together: a setting left out reads the row's random number instead
+    const float *none = reinterpret_cast<const float *>(a.u + r);
+    const float t0 = *(a.temperature ? a.temperature + r : none), p0 = *(a.top_p ? a.top_p + r : none), low0 = *(a.min_p ? a.min_p + r : none);
+    const int k0 = *(a.top_k ? a.top_k + r : reinterpret_cast<const int *>(none));
+    const float t = a.temperature ? t0 : 1.0f, p = a.top_p ? p0 : 0.f, low = a.min_p ? low0 : 0.f;
     RowAsks q;
-    q.k = a.top_k ? a.top_k[r] : 0;
+    q.k = a.top_k ? k0 : 0;
     q.greedy = !(t > 0.f) || q.k == 1;       // temperature 0: the largest, the lowest index among equals
     if (q.k < 0 || q.k >= a.vocab) q.k = 0;
     q.T = (double)t;
@@ -198,12 +222,10 @@ __global__ __launch_bounds__(kThreads) void sample_range_kernel(SampleArgs a, Sa
             if (v[j] > -INFINITY && v[j] < low) low = v[j];
         }
     }
-    for (int o = 32; o > 0; o >>= 1) {
-        const float t2 = __shfl_xor(top, o), l2 = __shfl_xor(low, o);
-        const int a2 = __shfl_xor(arg, o);
-        if (t2 > top || (t2 == top && a2 < arg)) { top = t2; arg = a2; }
-        low = fminf(low, l2);
-    }
+    const float wave_is = wave_top(top);
+    arg = wave_low(top == wave_is ? arg : INT32_MAX);
+    top = wave_is;
+    low = wave_low(low);
     if ((tid & 63) == 0) { tops[tid >> 6] = top; lows[tid >> 6] = low; args[tid >> 6] = arg; }
     __syncthreads();
     if (tid == 0) {
@@ -235,12 +257,10 @@ __device__ __forceinline__ RowRange row_range(const SampleWork &w, int row) {
         if (o.top > g.top) { g.top = o.top; g.arg = o.arg; }
         g.low = fminf(g.low, o.low);
     }
-    for (int o = 32; o > 0; o >>= 1) {
-        const float t2 = __shfl_xor(g.top, o), l2 = __shfl_xor(g.low, o);
-        const int a2 = __shfl_xor(g.arg, o);
-        if (t2 > g.top || (t2 == g.top && a2 < g.arg)) { g.top = t2; g.arg = a2; }
-        g.low = fminf(g.low, l2);
-    }
+    const float top = wave_top(g.top);
+    g.arg = wave_low(g.top == top ? g.arg : INT32_MAX);
+    g.top = top;
+    g.low = wave_low(g.low);
     return g;
 }
 
@@ -249,6 +269,9 @@ __global__ __launch_bounds__(kCountThreads) void sample_histogram_kernel(SampleA
     __shared__ uint32_t count[kBins];
     const int tid = threadIdx.x, split = blockIdx.x, row = blockIdx.y, r = w.row0 + row;
     const float *x = a.logits + (size_t)r * a.ld;
+    const int i0 = split * w.per_count, i1 = min(a.vocab, i0 + w.per_count);
+    float v[8];
+    load_steps(x, i0 + tid, kCountThreads, i1, v);                        // on their way while the rest is looked up
     const RowAsks q = row_asks(a, r);
     if (q.greedy || !(q.k > 0 || q.p > 0.f)) return;                      // no cut to find
     const RowRange g = row_range(w, row);
@@ -260,10 +283,9 @@ __global__ __launch_bounds__(kCountThreads) void sample_histogram_kernel(SampleA
         count[i] = 0;
     }
     __syncthreads();
-    const int i0 = split * w.per_count, i1 = min(a.vocab, i0 + w.per_count);
     for (int i = i0 + tid; i < i1; i += 8 * kCountThreads) {
-        float v[8];
-        load_steps(x, i, kCountThreads, i1, v);
+        float next[8];
+        load_steps(x, i + 8 * kCountThreads, kCountThreads, i1, next);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int bin = bin_of(b, v[j]);
@@ -271,6 +293,7 @@ __global__ __launch_bounds__(kCountThreads) void sample_histogram_kernel(SampleA
                 if (weighs) __hip_atomic_fetch_add(&sum[bin], whole(token_weight(b, v[j])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
                 __hip_atomic_fetch_add(&count[bin], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
             }
+            v[j] = next[j];
         }
     }
     __syncthreads();
@@ -310,52 +333,48 @@ __device__ __forceinline__ unsigned long long block_scan_u64(unsigned long long 
     return before + s - v;
 }
 
-// The bin in which the running weight (or count) of a row's histogram reaches a goal: `reaches(before, with)` says whether a piece
-// is that one.  One wave: the coarse bins, then the 64 bins of the one found.  -1: none.
-template <class V, class F>
-__device__ __forceinline__ int find_bin(const V *fine, unsigned long long coarse, F reaches, unsigned long long &before, unsigned long long &in) {
-    const int lane = (int)(threadIdx.x & 63);
-    const unsigned long long upto = wave_scan_u64(coarse), group = __ballot(reaches(upto - coarse, upto));
-    if (!group) return -1;
-    const int c = __builtin_amdgcn_readfirstlane(__ffsll(group) - 1);
-    const unsigned long long base = lane_u64(upto - coarse, c), its = fine[c * 64 + lane], run = base + wave_scan_u64(its);
-    const unsigned long long bin = __ballot(reaches(run - its, run));
-    const int l = __builtin_amdgcn_readfirstlane(bin ? __ffsll(bin) - 1 : 63);
-    before = lane_u64(run - its, l);
-    in = lane_u64(its, l);
-    return c * 64 + l;
+// Which of a wave's 64 pieces it is in which a running sum reaches a goal, by `reaches(before, with)`; 63 if it says so of none.
+template <class F>
+__device__ __forceinline__ int find_piece(unsigned long long before, unsigned long long with, F reaches) {
+    const unsigned long long is = __ballot(reaches(before, with));
+    return __builtin_amdgcn_readfirstlane(is ? __ffsll(is) - 1 : 63);
 }
 
-// The cuts' bins, from the row's histogram.  One wave calls this.
+// The cuts' bins, from the row's histogram: of the coarse bins the one, then of its 64 bins the one.  One wave calls this; two reads
+// that wait for one another behind the coarse bins, one where only one cut is asked for.
 __device__ RowBorders find_borders(const SampleWork &w, int row, const RowAsks &q) {
     const int lane = (int)(threadIdx.x & 63);
     const unsigned long long *sum = w.sum + (size_t)row * kBins;
-    const uint32_t *count = w.count + (size_t)row * kBins;
-    const unsigned long long coarse_sum = q.p > 0.f ? w.coarse_sum[(size_t)row * kCoarse + lane] : 0, coarse_count = w.coarse_count[(size_t)row * kCoarse + lane];
-    const unsigned long long all = wave_sum_u64(coarse_sum), tokens = wave_sum_u64(coarse_count);
+    const unsigned long long sums = q.p > 0.f ? w.coarse_sum[(size_t)row * kCoarse + lane] : 0, counts = w.coarse_count[(size_t)row * kCoarse + lane];
+    const unsigned long long sum_to = wave_scan_u64(sums), count_to = wave_scan_u64(counts), all = lane_u64(sum_to, 63), tokens = lane_u64(count_to, 63);
     RowBorders o{ all, all, all, 0, 0, q.k > 0 && (unsigned long long)q.k < tokens ? (unsigned long long)q.k : 0, 0, kBins, 0, -1, kBins };
-    unsigned long long in = 0;
     if (o.k) {
-        const unsigned long long k = o.k;
-        o.k_bin = find_bin(count, coarse_count, [k](unsigned long long from, unsigned long long to) { return from < k && k <= to; }, o.k_above, o.k_in);
-        if (q.p > 0.f) {
-            const int c = o.k_bin / 64, l = o.k_bin % 64;
-            const unsigned long long base = lane_u64(wave_scan_u64(coarse_sum) - coarse_sum, c), its = sum[c * 64 + lane], run = base + wave_scan_u64(its);
-            o.k_weight_above = lane_u64(run - its, l);
-            o.k_weight_with = lane_u64(run, l);
-        }
+        const auto holds_k = [k = o.k](unsigned long long from, unsigned long long to) { return from < k && k <= to; };
+        const int c = find_piece(count_to - counts, count_to, holds_k);
+        const unsigned long long n = w.count[(size_t)row * kBins + c * 64 + lane], s = q.p > 0.f ? sum[c * 64 + lane] : 0;
+        const unsigned long long n_to = lane_u64(count_to - counts, c) + wave_scan_u64(n), s_to = lane_u64(sum_to - sums, c) + wave_scan_u64(s);
+        const int l = find_piece(n_to - n, n_to, holds_k);
+        o.k_bin = c * 64 + l;
+        o.k_above = lane_u64(n_to - n, l);
+        o.k_in = lane_u64(n, l);
+        o.k_weight_above = lane_u64(s_to - s, l);
+        o.k_weight_with = lane_u64(s_to, l);
     }
     o.keep_below = o.k_bin;
     if (q.p > 0.f) {
         // the weight of the top k lies between that of the bins above its last one and that with it; nothing above: from bin 0 on
         const double lo = (double)q.p * (double)o.k_weight_above, hi = (double)q.p * (double)o.k_weight_with;
-        unsigned long long unused;
+        const auto reaches_lo = [lo](unsigned long long from, unsigned long long to) { return (double)from < lo && lo <= (double)to; };
+        const auto reaches_hi = [hi](unsigned long long from, unsigned long long to) { return (double)from < hi && hi <= (double)to; };
+        const int cl = find_piece(sum_to - sums, sum_to, reaches_lo), ch = find_piece(sum_to - sums, sum_to, reaches_hi);
+        const unsigned long long a = sum[cl * 64 + lane], b = sum[ch * 64 + lane];
+        const unsigned long long a_to = lane_u64(sum_to - sums, cl) + wave_scan_u64(a), b_to = lane_u64(sum_to - sums, ch) + wave_scan_u64(b);
         if (lo > 0.0) {
-            const int first = find_bin(sum, coarse_sum, [lo](unsigned long long from, unsigned long long to) { return (double)from < lo && lo <= (double)to; }, o.above_list, in);
-            o.p_first = max(first, 0);
+            const int l = find_piece(a_to - a, a_to, reaches_lo);
+            o.p_first = cl * 64 + l;
+            o.above_list = lane_u64(a_to - a, l);
         }
-        o.p_last = lo == hi ? o.p_first
-                            : find_bin(sum, coarse_sum, [hi](unsigned long long from, unsigned long long to) { return (double)from < hi && hi <= (double)to; }, unused, in);
+        o.p_last = ch * 64 + find_piece(b_to - b, b_to, reaches_hi);
         o.keep_below = o.p_first;
     }
     return o;
@@ -368,6 +387,9 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a, 
     __shared__ int n_found, place;
     const int tid = threadIdx.x, part = blockIdx.x, row = blockIdx.y, r = w.row0 + row;
     const float *x = a.logits + (size_t)r * a.ld;
+    const int i0 = part * kPart;
+    float v[kPart / kThreads];
+    load_steps(x, i0 + tid, kThreads, a.vocab, v);          // on their way while the borders are looked for
     const RowAsks q = row_asks(a, r);
     if (q.greedy) return;
     const RowRange g = row_range(w, row);
@@ -384,22 +406,17 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a, 
     if (part == 0 && tid == 0) w.borders[row] = borders;
     const int k_bin = borders.k_bin, p_first = borders.p_first, p_last = borders.p_last, keep_below = borders.keep_below;
     const double min_w = ldexp(q.min_w, a.frac_bits);
-    const int i0 = part * kPart, i1 = min(a.vocab, i0 + kPart);
     unsigned long long mine = 0;
-    for (int i = i0 + tid; i < i1; i += 8 * kThreads) {
-        float v[8];
-        load_steps(x, i, kThreads, i1, v);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int bin = bin_of(b, v[j]);
-            if (bin >= kBins) continue;
-            if (bin < keep_below) {
-                const double f = token_weight(b, v[j]);
-                if (f >= min_w) mine += whole(f);
-            } else if (bin == k_bin || (bin >= p_first && bin <= p_last)) {
-                const int at = __hip_atomic_fetch_add(&n_found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                if (at < kListMost) found[at] = rank_key(v[j], i + j * kThreads);
-            }
+    for (int j = 0; j < kPart / kThreads; j++) {
+        const int bin = bin_of(b, v[j]);
+        if (bin >= kBins) continue;
+        if (bin < keep_below) {
+            const double f = token_weight(b, v[j]);
+            if (f >= min_w) mine += whole(f);
+        } else if (bin == k_bin || (bin >= p_first && bin <= p_last)) {
+            const int at = __hip_atomic_fetch_add(&n_found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            if (at < kListMost) found[at] = rank_key(v[j], i0 + tid + j * kThreads);
         }
     }
     mine = block_sum_u64(mine, red);                        // its barriers also publish the list
