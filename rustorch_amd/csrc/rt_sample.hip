@@ -10,7 +10,7 @@
 // the draw do not depend on how the row is split over threads, and a token is lost to rounding only below 2^-(F+1) of the
 // largest weight (F = 45 for a vocabulary of 131072).  32-bit sums would move the cuts of a large vocabulary by whole tokens.
 //
-// Four launches.  sample_range_kernel finds each row's largest logit (and its smallest finite one), sample_histogram_kernel counts
+// Four launches.  sample_range_kernel finds each row's largest and smallest logit, sample_histogram_kernel counts
 // and weighs the tokens by how far below it they are, sample_collect_kernel finds from the histogram the bins that the cuts fall
 // into, lists the tokens of just those bins and sums the weights of the tokens above them, sample_finish_kernel ranks the listed
 // tokens exactly and draws.  The first three split a row over as many workgroups as fill the device.
@@ -100,13 +100,13 @@ __device__ __forceinline__ unsigned long long block_sum_u64(unsigned long long v
 }
 
 // ---- bins: a row's tokens by their distance d = M - l below the largest logit, up to the distance R beyond which the weight
-// rounds to zero (or the smallest finite logit, if that is nearer).  The bin's number is d * (kBins - 1) / R in f32: only its
+// rounds to zero (or the smallest logit, if that is nearer).  The bin's number is d * (kBins - 1) / R in f32: only its
 // being monotone in d matters, and that the last bin ends past R.
 // 4096 bins hold at most a hundred tokens each where the cuts of real rows fall; 1024 held several hundred, whose ranking (every
 // one against every other) took most of the time.
-constexpr int kBins = 4096, kThreads = 256, kCountThreads = 1024, kCoarse = kBins / 64, kListMost = 2048, kPart = 4096;
+constexpr int kBins = 4096, kThreads = 256, kCountThreads = 1024, kCoarse = kBins / 64, kListMost = 2048, kFewMost = kListMost / 2, kPart = 4096, kCountSort = 128;
 
-struct RowRange { float top, low; int arg, pad; };        // of one split of a row: largest logit, smallest finite one, index of the largest
+struct RowRange { float top, low; int arg, pad; };        // of one split of a row: largest and smallest logit; where only the largest counts, its index
 // What the histogram says of a row's cuts.
 struct RowBorders {
     unsigned long long all;                                // weight of the row
@@ -118,6 +118,7 @@ struct RowBorders {
     int p_first, p_last;                                   // the bins that top-p may end in (p_last = -1: no top-p)
     int keep_below;                                        // bins below this one stay whole
 };
+constexpr RowBorders kNoBorders{ 0, 0, 0, 0, 0, 0, 0, kBins, 0, -1, kBins };
 struct SampleWork {
     RowRange *range;                                       // [row][split]
     unsigned long long *sum;                               // [row][kBins]
@@ -147,8 +148,9 @@ __device__ __forceinline__ RowBins row_bins(float top, float low, double T, int 
     b.frac_bits = frac_bits;
     return b;
 }
-__device__ __forceinline__ int bin_of(const RowBins &b, float x) {       // kBins: beyond the reach, NaN or infinite
-    const float at = (b.half_top - 0.5f * x) * b.scale;
+__device__ __forceinline__ float bin_at(const RowBins &b, float x) { return (b.half_top - 0.5f * x) * b.scale; }      // NaN, or kBins and more: no bin
+__device__ __forceinline__ int bin_of(const RowBins &b, float x) {
+    const float at = bin_at(b, x);
     return at < (float)kBins ? (int)at : kBins;                          // false for NaN
 }
 // exp((x - M) / T) * 2^frac_bits in 64 bits: 2^t with t split into a whole number and |f| <= 1/2, the latter by the series of the
@@ -180,6 +182,7 @@ struct RowAsks {
     float p;                      // 0: off
     int k;                        // 0: off
     bool greedy;
+    bool few;                     // top-k so small that all its tokens are listed: nothing has to be weighed before
 };
 __device__ __forceinline__ RowAsks row_asks(const SampleArgs &a, int r) {
     // one load each, none behind a branch, so that they go out together: a setting left out reads the row's random number instead
@@ -191,17 +194,57 @@ __device__ __forceinline__ RowAsks row_asks(const SampleArgs &a, int r) {
     q.k = a.top_k ? k0 : 0;
     q.greedy = !(t > 0.f) || q.k == 1;       // temperature 0: the largest, the lowest index among equals
     if (q.k < 0 || q.k >= a.vocab) q.k = 0;
+    q.few = q.k > 0 && q.k <= kFewMost;
     q.T = (double)t;
     q.p = p > 0.f && p < 1.f ? p : 0.f;
     q.min_w = low > 0.f ? fmin((double)low, 1.0) : 0.0;
     return q;
 }
 
-// N values of a row, `step` apart from i on; NaN from `end` on.  The requests go out together.
-template <int N>
-__device__ __forceinline__ void load_steps(const float *x, int i, int step, int end, float (&v)[N]) {
+// the range of all lanes' ranges
+__device__ __forceinline__ void fold_range(RowRange &g) {
+    const float top = wave_top(g.top);
+    g.arg = wave_low(g.top == top ? g.arg : INT32_MAX);
+    g.top = top;
+    g.low = wave_low(g.low);
+}
+// A row with nothing to draw from, or nothing to draw: written here.
+__device__ __forceinline__ bool undrawn_row(const SampleArgs &a, int r, const RowAsks &q, const RowRange &g) {
+    if (g.top != -INFINITY && !q.greedy) return false;
+    if (threadIdx.x == 0) {
+        a.out_token[r] = g.top == -INFINITY ? -1 : g.arg;
+        if (a.out_prob) a.out_prob[r] = g.top == -INFINITY ? 0.f : 1.f;
+    }
+    return true;
+}
+
+// N values, STEP apart, of a row of which `left` are left from x on (the same for all threads); NaN behind its end.  The requests
+// go out together.
+template <int N, int STEP>
+__device__ __forceinline__ void load_steps(const float *x, int left, float (&v)[N]) {
+    const unsigned tid = threadIdx.x;
+    if (left >= N * STEP) {
 #pragma unroll
-    for (int j = 0; j < N; j++) v[j] = i + j * step < end ? x[i + j * step] : NAN;
+        for (int j = 0; j < N; j++) v[j] = (x + j * STEP)[tid];
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; j++) v[j] = (int)tid + j * STEP < left ? (x + j * STEP)[tid] : NAN;
+    }
+}
+
+// The lowest index at which the n values from x on are equal to `top`, counted from `from`; INT32_MAX for none.  STEP threads.
+template <int STEP>
+__device__ __forceinline__ int first_of(const float *x, int n, int from, float top) {
+    int arg = INT32_MAX;
+#pragma unroll 1
+    for (int i = 0; i < n; i += 8 * STEP) {
+        float v[8];
+        load_steps<8, STEP>(x + i, n - i, v);
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (v[j] == top) arg = min(arg, from + i + j * STEP + (int)threadIdx.x);
+    }
+    return arg;
 }
 
 // The range of one split of a row; also clears the split's share of the row's histogram.
@@ -210,29 +253,32 @@ __global__ __launch_bounds__(kThreads) void sample_range_kernel(SampleArgs a, Sa
     __shared__ int args[4];
     const int tid = threadIdx.x, split = blockIdx.x, row = blockIdx.y, r = w.row0 + row;
     const float *x = a.logits + (size_t)r * a.ld;
-    const int i0 = split * w.per_split, i1 = min(a.vocab, i0 + w.per_split);
+    const int i0 = split * w.per_split, n = max(0, min(a.vocab, i0 + w.per_split) - i0);
     float top = -INFINITY, low = INFINITY;
-    int arg = INT32_MAX;
-    for (int i = i0 + tid; i < i1; i += 8 * 256) {
+    for (int i = 0; i < n; i += 8 * kThreads) {
         float v[8];
-        load_steps(x, i, 256, i1, v);
+        load_steps<8, kThreads>(x + i0 + i, n - i, v);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            if (v[j] > top) { top = v[j]; arg = i + 256 * j; }          // NaN: false; ascending index: the lowest of equals
-            if (v[j] > -INFINITY && v[j] < low) low = v[j];
+            top = fmaxf(top, v[j]);                             // NaN: neither
+            low = fminf(low, v[j]);
         }
     }
-    const float wave_is = wave_top(top);
-    arg = wave_low(top == wave_is ? arg : INT32_MAX);
-    top = wave_is;
+    top = wave_top(top);
     low = wave_low(low);
-    if ((tid & 63) == 0) { tops[tid >> 6] = top; lows[tid >> 6] = low; args[tid >> 6] = arg; }
+    if ((tid & 63) == 0) { tops[tid >> 6] = top; lows[tid >> 6] = low; }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; i++) {
+        top = fmaxf(top, tops[i]);
+        low = fminf(low, lows[i]);
+    }
+    int arg = row_asks(a, r).greedy ? first_of<kThreads>(x + i0, n, i0, top) : INT32_MAX;
+    arg = wave_low(arg);
+    if ((tid & 63) == 0) args[tid >> 6] = arg;
     __syncthreads();
     if (tid == 0) {
-        for (int i = 1; i < 4; i++) {
-            if (tops[i] > top || (tops[i] == top && args[i] < arg)) { top = tops[i]; arg = args[i]; }
-            low = fminf(low, lows[i]);
-        }
+        for (int i = 1; i < kThreads / 64; i++) arg = min(arg, args[i]);
         w.range[(size_t)row * w.splits + split] = RowRange{ top, low, arg, 0 };
     }
     if (split == 0) {
@@ -257,10 +303,7 @@ __device__ __forceinline__ RowRange row_range(const SampleWork &w, int row) {
         if (o.top > g.top) { g.top = o.top; g.arg = o.arg; }
         g.low = fminf(g.low, o.low);
     }
-    const float top = wave_top(g.top);
-    g.arg = wave_low(g.top == top ? g.arg : INT32_MAX);
-    g.top = top;
-    g.low = wave_low(g.low);
+    fold_range(g);
     return g;
 }
 
@@ -269,23 +312,23 @@ __global__ __launch_bounds__(kCountThreads) void sample_histogram_kernel(SampleA
     __shared__ uint32_t count[kBins];
     const int tid = threadIdx.x, split = blockIdx.x, row = blockIdx.y, r = w.row0 + row;
     const float *x = a.logits + (size_t)r * a.ld;
-    const int i0 = split * w.per_count, i1 = min(a.vocab, i0 + w.per_count);
+    const int i0 = split * w.per_count, n = max(0, min(a.vocab, i0 + w.per_count) - i0);
     float v[8];
-    load_steps(x, i0 + tid, kCountThreads, i1, v);                        // on their way while the rest is looked up
+    load_steps<8, kCountThreads>(x + i0, n, v);                           // on their way while the rest is looked up
     const RowAsks q = row_asks(a, r);
     if (q.greedy || !(q.k > 0 || q.p > 0.f)) return;                      // no cut to find
     const RowRange g = row_range(w, row);
     if (g.top == -INFINITY || g.top == INFINITY) return;                  // without weights
-    const bool weighs = q.p > 0.f;                                        // top-k alone counts
+    const bool weighs = q.p > 0.f && !q.few;                              // top-k alone counts
     const RowBins b = row_bins(g.top, g.low, q.T, a.frac_bits);
     for (int i = tid; i < kBins; i += kCountThreads) {
         sum[i] = 0;
         count[i] = 0;
     }
     __syncthreads();
-    for (int i = i0 + tid; i < i1; i += 8 * kCountThreads) {
+    for (int i = 0; i < n; i += 8 * kCountThreads) {
         float next[8];
-        load_steps(x, i + 8 * kCountThreads, kCountThreads, i1, next);
+        load_steps<8, kCountThreads>(x + i0 + i + 8 * kCountThreads, n - i - 8 * kCountThreads, next);
 #pragma unroll
         for (int j = 0; j < 8; j++) {
             const int bin = bin_of(b, v[j]);
@@ -342,16 +385,17 @@ __device__ __forceinline__ int find_piece(unsigned long long before, unsigned lo
 
 // The cuts' bins, from the row's histogram: of the coarse bins the one, then of its 64 bins the one.  One wave calls this; two reads
 // that wait for one another behind the coarse bins, one where only one cut is asked for.
-__device__ RowBorders find_borders(const SampleWork &w, int row, const RowAsks &q) {
+__device__ RowBorders find_borders(const unsigned long long *sum, const uint32_t *count, const unsigned long long *coarse_sum, const uint32_t *coarse_count,
+                                   const RowAsks &q) {
     const int lane = (int)(threadIdx.x & 63);
-    const unsigned long long *sum = w.sum + (size_t)row * kBins;
-    const unsigned long long sums = q.p > 0.f ? w.coarse_sum[(size_t)row * kCoarse + lane] : 0, counts = w.coarse_count[(size_t)row * kCoarse + lane];
+    const bool weighed = q.p > 0.f && !q.few;
+    const unsigned long long sums = weighed ? coarse_sum[lane] : 0, counts = coarse_count[lane];
     const unsigned long long sum_to = wave_scan_u64(sums), count_to = wave_scan_u64(counts), all = lane_u64(sum_to, 63), tokens = lane_u64(count_to, 63);
-    RowBorders o{ all, all, all, 0, 0, q.k > 0 && (unsigned long long)q.k < tokens ? (unsigned long long)q.k : 0, 0, kBins, 0, -1, kBins };
+    RowBorders o{ all, all, all, 0, 0, q.k > 0 && (unsigned long long)q.k < tokens ? (unsigned long long)q.k : (q.few ? tokens : 0), 0, kBins, 0, -1, kBins };
     if (o.k) {
         const auto holds_k = [k = o.k](unsigned long long from, unsigned long long to) { return from < k && k <= to; };
         const int c = find_piece(count_to - counts, count_to, holds_k);
-        const unsigned long long n = w.count[(size_t)row * kBins + c * 64 + lane], s = q.p > 0.f ? sum[c * 64 + lane] : 0;
+        const unsigned long long n = count[c * 64 + lane], s = weighed ? sum[c * 64 + lane] : 0;
         const unsigned long long n_to = lane_u64(count_to - counts, c) + wave_scan_u64(n), s_to = lane_u64(sum_to - sums, c) + wave_scan_u64(s);
         const int l = find_piece(n_to - n, n_to, holds_k);
         o.k_bin = c * 64 + l;
@@ -361,7 +405,12 @@ __device__ RowBorders find_borders(const SampleWork &w, int row, const RowAsks &
         o.k_weight_with = lane_u64(s_to, l);
     }
     o.keep_below = o.k_bin;
-    if (q.p > 0.f) {
+    if (q.few) {                                            // the list holds every token down to the last of the top k
+        o.k_in += o.k_above;
+        o.k_above = 0;
+        o.p_last = o.k_bin;
+        o.keep_below = 0;
+    } else if (q.p > 0.f) {
         // the weight of the top k lies between that of the bins above its last one and that with it; nothing above: from bin 0 on
         const double lo = (double)q.p * (double)o.k_weight_above, hi = (double)q.p * (double)o.k_weight_with;
         const auto reaches_lo = [lo](unsigned long long from, unsigned long long to) { return (double)from < lo && lo <= (double)to; };
@@ -380,6 +429,15 @@ __device__ RowBorders find_borders(const SampleWork &w, int row, const RowAsks &
     return o;
 }
 
+// The same borders as a token's place among the bins meets them.
+struct Wanted {
+    float keep, p0, p1, k0, k1;
+    __device__ explicit Wanted(const RowBorders &c)
+        : keep((float)c.keep_below), p0((float)c.p_first), p1((float)(c.p_last + 1)), k0((float)c.k_bin), k1(c.k_bin < kBins ? (float)(c.k_bin + 1) : 0.f) {}
+    __device__ bool kept(float at) const { return at < keep; }
+    __device__ bool listed(float at) const { return (at >= p0 && at < p1) || (at >= k0 && at < k1); }
+};
+
 // One workgroup per kPart tokens of a row: lists the tokens of the cuts' bins and sums the weights of the tokens above them.
 __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a, SampleWork w) {
     __shared__ unsigned long long found[kListMost], red[kThreads / 64];
@@ -389,14 +447,16 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a, 
     const float *x = a.logits + (size_t)r * a.ld;
     const int i0 = part * kPart;
     float v[kPart / kThreads];
-    load_steps(x, i0 + tid, kThreads, a.vocab, v);          // on their way while the borders are looked for
+    load_steps<kPart / kThreads, kThreads>(x + i0, a.vocab - i0, v);      // on their way while the borders are looked for
     const RowAsks q = row_asks(a, r);
     if (q.greedy) return;
     const RowRange g = row_range(w, row);
     if (g.top == -INFINITY || g.top == INFINITY) return;
     const RowBins b = row_bins(g.top, g.low, q.T, a.frac_bits);
     if (tid < 64) {
-        const RowBorders o = q.k > 0 || q.p > 0.f ? find_borders(w, row, q) : RowBorders{ 0, 0, 0, 0, 0, 0, 0, kBins, 0, -1, kBins };
+        const RowBorders o = q.k > 0 || q.p > 0.f ? find_borders(w.sum + (size_t)row * kBins, w.count + (size_t)row * kBins, w.coarse_sum + (size_t)row * kCoarse,
+                                                                 w.coarse_count + (size_t)row * kCoarse, q)
+                                                  : kNoBorders;
         if (tid == 0) {
             borders = o;
             n_found = 0;
@@ -404,19 +464,18 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a, 
     }
     __syncthreads();
     if (part == 0 && tid == 0) w.borders[row] = borders;
-    const int k_bin = borders.k_bin, p_first = borders.p_first, p_last = borders.p_last, keep_below = borders.keep_below;
+    const Wanted want(borders);
     const double min_w = ldexp(q.min_w, a.frac_bits);
     unsigned long long mine = 0;
 #pragma unroll
     for (int j = 0; j < kPart / kThreads; j++) {
-        const int bin = bin_of(b, v[j]);
-        if (bin >= kBins) continue;
-        if (bin < keep_below) {
+        const float at = bin_at(b, v[j]);
+        if (want.kept(at)) {
             const double f = token_weight(b, v[j]);
             if (f >= min_w) mine += whole(f);
-        } else if (bin == k_bin || (bin >= p_first && bin <= p_last)) {
-            const int at = __hip_atomic_fetch_add(&n_found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            if (at < kListMost) found[at] = rank_key(v[j], i0 + tid + j * kThreads);
+        } else if (want.listed(at)) {
+            const int place = __hip_atomic_fetch_add(&n_found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+            if (place < kListMost) found[place] = rank_key(v[j], i0 + tid + j * kThreads);
         }
     }
     mine = block_sum_u64(mine, red);                        // its barriers also publish the list
@@ -432,7 +491,8 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a, 
 
 // The row on its own, without bins: the cuts by bisection over the 32 bits of the logits' order, one pass over the row per bit.
 // For rows with infinite logits and for rows with more equal or nearly equal logits in one bin than the list of
-// sample_finish_kernel holds.  run: kThreads entries, tie as many.
+// finish_row holds.  run: kThreads entries, tie as many.
+template <int kThreads>
 __device__ void sample_by_bisection(const SampleArgs &a, int r, const RowAsks &q, float top, unsigned long long *run, int *tie, unsigned long long *red) {
     const int tid = threadIdx.x, V = a.vocab, k = q.k > 0 ? q.k : V;
     const float *x = a.logits + (size_t)r * a.ld;
@@ -535,137 +595,111 @@ __device__ void sample_by_bisection(const SampleArgs &a, int r, const RowAsks &q
     }
 }
 
-__global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, SampleWork w) {
-    constexpr int kMine = kListMost / kThreads, kOwn = kPart / kThreads;
-    __shared__ unsigned long long buf[kPart];               // the list's keys and weights; the weights of one part; bisection's scratch
-    __shared__ unsigned long long red[kThreads / 64], shared64[2];
+// The end of a row: ranks the listed tokens, finds the last one that stays, draws.  buf: kPart entries, the list's keys in the
+// first n_list; parts: the weight that stays whole of each kPart tokens, n_parts <= kThreads of them.  The whole workgroup calls this.
+// Loops stay loops here and below: this code runs once per row, and straight-line code of tens of kilobytes is paid for in
+// instruction fetches (one row of 1000 tokens, no filter: 13.4 us with 82 KB of code, 8.2 us with 34 KB).
+template <int kThreads>
+__device__ __forceinline__ void finish_row(const SampleArgs &a, int r, const RowAsks &q, const RowBins &b, const RowBorders &c, int n_list, unsigned long long *buf,
+                                           unsigned long long *parts, int n_parts, unsigned long long *red) {
+    constexpr int kOwn = kPart / kThreads;
+    __shared__ unsigned long long found_cut, before_chosen;
     __shared__ int chosen;
-    static_assert(2 * kListMost <= kPart && kOwn <= kThreads, "the list fits the buffer");
-    unsigned long long *list = buf, *list_weight = buf + kListMost;
-    const int tid = threadIdx.x, row = blockIdx.x, r = w.row0 + row, V = a.vocab;
+    static_assert(2 * kListMost <= kPart && kListMost >= 2 * kCountSort && kThreads >= kCountSort, "what buf is used for");
+    unsigned long long *upto = buf + kListMost;             // running weight of the sorted list, each token's own included
+    const int tid = threadIdx.x, V = a.vocab;
     const float *x = a.logits + (size_t)r * a.ld;
-    const RowAsks q = row_asks(a, r);
-    const RowRange g = row_range(w, row);
-    if (g.top == -INFINITY || q.greedy) {                   // nothing to draw from, or nothing to draw
-        if (tid == 0) {
-            a.out_token[r] = g.top == -INFINITY ? -1 : g.arg;
-            if (a.out_prob) a.out_prob[r] = g.top == -INFINITY ? 0.f : 1.f;
-        }
-        return;
-    }
-    const int n_list = g.top == INFINITY ? 0 : w.listed[row];
-    if (g.top == INFINITY || n_list > kListMost) {
-        sample_by_bisection(a, r, q, g.top, buf, reinterpret_cast<int *>(buf + kThreads), red);
-        return;
-    }
-    const RowBins b = row_bins(g.top, g.low, q.T, a.frac_bits);
-    const RowBorders c = w.borders[row];
     const double min_w = ldexp(q.min_w, a.frac_bits);
 
     // ---- the last key that stays
     unsigned long long cut = ~0ull;
-    unsigned long long key[kMine], own[kMine];
     if (n_list > 0) {
-        unsigned long long weight_before[kMine];
-        int rank[kMine];
-#pragma unroll
-        for (int m = 0; m < kMine; m++) {
-            const int i = tid + m * kThreads;
-            key[m] = own[m] = weight_before[m] = 0;
-            rank[m] = 0;
-            if (i < n_list) {
-                key[m] = w.list[(size_t)row * kListMost + i];
-                const float v = order_logit(~(uint32_t)(key[m] >> 32));
-                own[m] = whole(token_weight(b, v));
-                list[i] = key[m];
-                list_weight[i] = own[m];
-            }
+        if (n_list <= kCountSort) {          // sorted by counting the keys before each
+            const unsigned long long mine = tid < n_list ? buf[tid] : 0;
+            int rank = 0;
+#pragma unroll 4
+            for (int j = 0; j < n_list; j++) rank += buf[j] < mine ? 1 : 0;
+            __syncthreads();
+            if (tid < n_list) buf[rank] = mine;
+            __syncthreads();
+        } else {                             // bitonic sort: log2(span) * (log2(span) + 1) / 2 steps of span / 2 exchanges
+            int span = 2 * kCountSort;
+            while (span < n_list) span <<= 1;
+            for (int i = n_list + tid; i < span; i += kThreads) buf[i] = ~0ull;
+            __syncthreads();
+            for (int size = 2; size <= span; size <<= 1)
+                for (int stride = size >> 1; stride > 0; stride >>= 1) {
+                    for (int t = tid; t < span / 2; t += kThreads) {
+                        const int i = 2 * t - (t & (stride - 1)), o = i + stride;
+                        const unsigned long long x0 = buf[i], x1 = buf[o];
+                        if ((x0 > x1) == ((i & size) == 0)) {
+                            buf[i] = x1;
+                            buf[o] = x0;
+                        }
+                    }
+                    __syncthreads();
+                }
+        }
+        unsigned long long run = 0;
+#pragma unroll 1
+        for (int i0 = 0; i0 < n_list; i0 += kThreads) {
+            const int i = i0 + tid;
+            const unsigned long long weight = i < n_list ? whole(token_weight(b, order_logit(~(uint32_t)(buf[i] >> 32)))) : 0;
+            unsigned long long sum;
+            const unsigned long long before = run + block_scan_u64(weight, red, sum);
+            if (i < n_list) upto[i] = before + weight;
+            run += sum;
         }
         __syncthreads();
-        // every listed token's number and weight of listed tokens before it.  The listed bins are top-p's, one after the other, and
-        // top-k's, which is the last of them or comes behind them.
-        // (eight at a time: the reads of LDS go out together)
-        for (int j0 = 0; j0 < n_list; j0 += 8) {
-            unsigned long long other[8], its[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                other[j] = j0 + j < n_list ? list[j0 + j] : ~0ull;
-                its[j] = list_weight[j0 + j];
-            }
-#pragma unroll
-            for (int m = 0; m < kMine; m++)
-                if (m * kThreads < n_list) {
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if (other[j] < key[m]) {
-                            rank[m]++;
-                            weight_before[m] += its[j];
-                        }
-                }
-        }
+        // the listed bins are top-p's, one after the other, and top-k's, which is the last of them or comes behind them
         double goal = (double)q.p * (double)c.all;
+        int stay = n_list;
         if (c.k) {
-            unsigned long long mine = 0;
-            const int k_from = n_list - (int)c.k_in;        // where the list's part in the bin of top-k begins
-#pragma unroll
-            for (int m = 0; m < kMine; m++)
-                if (tid + m * kThreads < n_list && rank[m] >= k_from) {
-                    const unsigned long long nth = c.k_above + (unsigned long long)(rank[m] - k_from);
-                    if (nth < c.k) mine += own[m];
-                    if (nth == c.k - 1) shared64[0] = key[m];
-                }
-            mine = block_sum_u64(mine, red);                // its barriers publish shared64[0]
-            cut = shared64[0];
-            goal = (double)q.p * (double)(c.k_weight_above + mine);
+            const int k_from = n_list - (int)c.k_in;        // the list's part in the bin of top-k
+            stay = k_from + (int)(c.k - c.k_above);
+            cut = buf[stay - 1];
+            goal = (double)q.p * (double)(c.k_weight_above + upto[stay - 1] - (k_from > 0 ? upto[k_from - 1] : 0));
         }
         if (q.p > 0.f) {
             // the first token at which the weight reaches the goal; it is one of the listed, and not behind top-k's last
-#pragma unroll
-            for (int m = 0; m < kMine; m++)
-                if (tid + m * kThreads < n_list && key[m] <= cut) {
-                    const unsigned long long before = c.above_list + weight_before[m];
-                    if ((double)before < goal && (double)(before + own[m]) >= goal) shared64[1] = key[m];
-                }
-            __syncthreads();
-            cut = shared64[1];
-        }
-        __syncthreads();                                    // the list's memory is free from here on
-    }
-
-    // ---- the draw, by index, over the tokens whose key is at most the cut: which part, then which token of it.  What stays of the
-    // listed tokens joins the parts' sums first.
-    for (int p = tid; p < w.parts; p += kThreads) buf[p] = w.part_sum[(size_t)row * w.parts + p];
-    __syncthreads();
-    if (n_list > 0) {
-#pragma unroll
-        for (int m = 0; m < kMine; m++)
-            if (tid + m * kThreads < n_list && key[m] <= cut) {
-                const float v = order_logit(~(uint32_t)(key[m] >> 32));
-                if (token_weight(b, v) >= min_w)
-                    __hip_atomic_fetch_add(&buf[(uint32_t)key[m] / kPart], own[m], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+#pragma unroll 1
+            for (int i = tid; i < stay; i += kThreads) {
+                const unsigned long long before = c.above_list + (i > 0 ? upto[i - 1] : 0);
+                if ((double)before < goal && (double)(c.above_list + upto[i]) >= goal) found_cut = buf[i];
             }
-        __syncthreads();
+            __syncthreads();
+            cut = found_cut;
+        }
+        // what stays of the listed tokens joins the parts' sums
+#pragma unroll 1
+        for (int i = tid; i < n_list; i += kThreads) {
+            const unsigned long long key = buf[i];
+            const double f = token_weight(b, order_logit(~(uint32_t)(key >> 32)));
+            if (key <= cut && f >= min_w) __hip_atomic_fetch_add(&parts[(uint32_t)key / kPart], whole(f), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
     }
+    __syncthreads();                                        // the list's memory is free from here on
+
+    // ---- the draw, by index, over the tokens whose key is at most the cut: which part, then which token of it
     unsigned long long total;
-    const unsigned long long part = tid < w.parts ? buf[tid] : 0, before_part = block_scan_u64(part, red, total);      // at most kThreads parts
+    const unsigned long long part = tid < n_parts ? parts[tid] : 0, before_part = block_scan_u64(part, red, total);
     const double u = fmin(fmax(a.u[r], 0.0), 1.0);          // NaN: 0
     unsigned long long goal = (unsigned long long)floor(u * (double)total);      // the first token with (running weight) > goal
     if (goal >= total) goal = total - 1;
     if (part && before_part <= goal && goal < before_part + part) {
         chosen = tid;
-        shared64[0] = before_part;
+        before_chosen = before_part;
     }
     __syncthreads();
     const int i0 = chosen * kPart;
-    unsigned long long before = shared64[0];
-    float v[kOwn];
-    load_steps(x, i0 + tid, kThreads, V, v);
-#pragma unroll
+#pragma unroll 4
     for (int j = 0; j < kOwn; j++) {
-        const int i = i0 + j * kThreads + tid, bin = bin_of(b, v[j]);
+        const int i = i0 + j * kThreads + tid;
+        const float v = i < V ? x[i] : NAN;
+        const int bin = bin_of(b, v);
         unsigned long long weight = 0;
-        if (bin < kBins && rank_key(v[j], i) <= cut) {
-            const double f = token_weight(b, v[j]);
+        if (bin < kBins && rank_key(v, i) <= cut) {
+            const double f = token_weight(b, v);
             if (f >= min_w) weight = whole(f);
         }
         buf[j * kThreads + tid] = weight;
@@ -674,8 +708,9 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, S
     // a thread per kOwn consecutive tokens
     unsigned long long mine = 0, sum;
     for (int j = 0; j < kOwn; j++) mine += buf[tid * kOwn + j];
-    unsigned long long at = before + block_scan_u64(mine, red, sum);
+    unsigned long long at = before_chosen + block_scan_u64(mine, red, sum);
     if (mine && at <= goal && goal < at + mine)
+#pragma unroll 1
         for (int j = 0; j < kOwn; j++) {
             const unsigned long long weight = buf[tid * kOwn + j];
             if (weight && goal < at + weight) {
@@ -686,6 +721,142 @@ __global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, S
             }
             at += weight;
         }
+}
+
+__global__ __launch_bounds__(kThreads) void sample_finish_kernel(SampleArgs a, SampleWork w) {
+    __shared__ unsigned long long buf[kPart], parts[kThreads], red[kThreads / 64];
+    const int tid = threadIdx.x, row = blockIdx.x, r = w.row0 + row;
+    const unsigned long long part = tid < w.parts ? w.part_sum[(size_t)row * w.parts + tid] : 0;      // at most kThreads parts
+    const RowAsks q = row_asks(a, r);
+    const RowRange g = row_range(w, row);
+    const int n_list = w.listed[row];
+    if (undrawn_row(a, r, q, g)) return;
+    if (g.top == INFINITY || n_list > kListMost) {
+        sample_by_bisection<kThreads>(a, r, q, g.top, buf, reinterpret_cast<int *>(buf + kThreads), red);
+        return;
+    }
+    const RowBorders c = w.borders[row];
+    parts[tid] = part;
+    for (int i = tid; i < n_list; i += kThreads) buf[i] = w.list[(size_t)row * kListMost + i];
+    __syncthreads();
+    finish_row<kThreads>(a, r, q, row_bins(g.top, g.low, q.T, a.frac_bits), c, n_list, buf, parts, w.parts, red);
+}
+
+// ---- the whole of it by one workgroup per row, in one launch: the row is read three times, the last two from the L2.
+constexpr int kRowThreads = 1024, kStep = 8;
+__global__ __launch_bounds__(kRowThreads) void sample_row_kernel(SampleArgs a) {
+    __shared__ unsigned long long sum[kBins], coarse_sum[kCoarse], parts[kThreads + kStep / 4], red[kRowThreads / 64];
+    __shared__ uint32_t count[kBins], coarse_count[kCoarse];
+    __shared__ RowBorders borders;
+    __shared__ float tops[kRowThreads / 64], lows[kRowThreads / 64];
+    __shared__ int args[kRowThreads / 64], n_found;
+    static_assert(kBins >= kPart && kPart == 4 * kRowThreads, "the list takes the histogram's place; four steps are a part");
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = blockIdx.x, n_parts = (a.vocab + kPart - 1) / kPart;
+    const float *x = a.logits + (size_t)r * a.ld;
+    const RowAsks q = row_asks(a, r);
+    for (int i = tid; i < kBins; i += kRowThreads) {
+        sum[i] = 0;
+        count[i] = 0;
+    }
+    if (tid < kThreads) parts[tid] = 0;
+    if (tid == 0) n_found = 0;
+    RowRange g{ -INFINITY, INFINITY, INT32_MAX, 0 };
+    float v[kStep], next[kStep];             // the next step's values are on their way while a step's are used
+    load_steps<kStep, kRowThreads>(x, a.vocab, v);
+#pragma unroll 1
+    for (int i0 = 0; i0 < a.vocab; i0 += kStep * kRowThreads) {
+        load_steps<kStep, kRowThreads>(x + i0 + kStep * kRowThreads, a.vocab - i0 - kStep * kRowThreads, next);
+#pragma unroll
+        for (int j = 0; j < kStep; j++) {
+            g.top = fmaxf(g.top, v[j]);                          // NaN: neither
+            g.low = fminf(g.low, v[j]);
+            v[j] = next[j];
+        }
+    }
+    load_steps<kStep, kRowThreads>(x, a.vocab, v);
+    g.top = wave_top(g.top);
+    g.low = wave_low(g.low);
+    if (lane == 0) { tops[wave] = g.top; lows[wave] = g.low; }
+    __syncthreads();
+    g.top = wave_top(lane < kRowThreads / 64 ? tops[lane] : -INFINITY);
+    g.low = wave_low(lane < kRowThreads / 64 ? lows[lane] : INFINITY);
+    if (q.greedy) {
+        g.arg = wave_low(first_of<kRowThreads>(x, a.vocab, 0, g.top));
+        if (lane == 0) args[wave] = g.arg;
+        __syncthreads();
+        g.arg = wave_low(lane < kRowThreads / 64 ? args[lane] : INT32_MAX);
+    }
+    if (undrawn_row(a, r, q, g)) return;
+    int n_list = g.top == INFINITY ? kListMost + 1 : 0;
+    if (n_list == 0) {
+        const RowBins b = row_bins(g.top, g.low, q.T, a.frac_bits);
+        const bool cuts = q.k > 0 || q.p > 0.f, weighs = q.p > 0.f && !q.few;
+        if (cuts) {
+#pragma unroll 1
+            for (int i0 = 0; i0 < a.vocab; i0 += kStep * kRowThreads) {
+                load_steps<kStep, kRowThreads>(x + i0 + kStep * kRowThreads, a.vocab - i0 - kStep * kRowThreads, next);
+#pragma unroll
+                for (int j = 0; j < kStep; j++) {
+                    const int bin = bin_of(b, v[j]);
+                    if (bin < kBins) {
+                        if (weighs) __hip_atomic_fetch_add(&sum[bin], whole(token_weight(b, v[j])), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                        __hip_atomic_fetch_add(&count[bin], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                    }
+                    v[j] = next[j];
+                }
+            }
+            load_steps<kStep, kRowThreads>(x, a.vocab, v);
+            __syncthreads();
+#pragma unroll 1
+            for (int i = tid; i < kBins; i += kRowThreads) {              // a wave has the 64 bins of one coarse bin
+                const unsigned long long n = wave_sum_u64(count[i]), s = weighs ? wave_sum_u64(sum[i]) : 0;
+                if (lane == 0) {
+                    coarse_count[i / 64] = (uint32_t)n;
+                    coarse_sum[i / 64] = s;
+                }
+            }
+            __syncthreads();
+            if (wave == 0) {
+                const RowBorders o = find_borders(sum, count, coarse_sum, coarse_count, q);
+                if (lane == 0) borders = o;
+            }
+        } else if (tid == 0) {
+            borders = kNoBorders;
+        }
+        __syncthreads();                                    // the histogram's memory takes the list from here on
+        const RowBorders c = borders;
+        const Wanted want(c);
+        const double min_w = ldexp(q.min_w, a.frac_bits);
+#pragma unroll 1
+        for (int i0 = 0; i0 < a.vocab; i0 += kStep * kRowThreads) {
+            load_steps<kStep, kRowThreads>(x + i0 + kStep * kRowThreads, a.vocab - i0 - kStep * kRowThreads, next);
+            unsigned long long mine = 0;
+#pragma unroll
+            for (int j = 0; j < kStep; j++) {
+                const float at = bin_at(b, v[j]);
+                if (want.kept(at)) {
+                    const double f = token_weight(b, v[j]);
+                    if (f >= min_w) mine += whole(f);
+                } else if (want.listed(at)) {
+                    const int place = __hip_atomic_fetch_add(&n_found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                    if (place < kListMost) sum[place] = rank_key(v[j], i0 + tid + j * kRowThreads);
+                }
+                v[j] = next[j];
+                if (c.keep_below > 0 && j % 4 == 3) {       // the end of a part
+                    mine = wave_sum_u64(mine);
+                    if (lane == 0 && mine) __hip_atomic_fetch_add(&parts[i0 / kPart + j / 4], mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                    mine = 0;
+                }
+            }
+        }
+        __syncthreads();
+        n_list = n_found;
+        if (n_list <= kListMost) {
+            finish_row<kRowThreads>(a, r, q, b, c, n_list, sum, parts, n_parts, red);
+            return;
+        }
+    }
+    sample_by_bisection<kRowThreads>(a, r, q, g.top, sum, reinterpret_cast<int *>(count), red);
 }
 
 }  // namespace
@@ -709,6 +880,15 @@ int rt_hip_sample_dev(rt_hip_ctx *ctx, const float *logits, size_t ld, int n_row
     int bits = 0;
     while ((1 << bits) < vocab) bits++;
     rt::SampleArgs a{ logits, ld, n_rows, vocab, bits < 11 ? 51 : 62 - bits, u, temperature, top_p, min_p, top_k, out_token, out_prob };
+    // One workgroup per row, or rows split over the device in four launches (us; top-k 40 and top-p 0.95 / top-p 0.9 / no filter):
+    //   rows x vocab    1 x 32000   64 x 32000  256 x 32000  64 x 65536  77 x 131071  1 x 131071
+    //   one launch      23/42/23    24/44/24    28/47/27     34/73/39    59/135/73    50/127/65
+    //   four            26/31/21    40/55/27    55/78/42     46/63/31    62/94/44     30/36/20
+    if (vocab <= 32768) {
+        rt::sample_row_kernel<<<dim3((unsigned)n_rows), rt::kRowThreads, 0, ctx->stream>>>(a);
+        RT_TRY_HIP(ctx, hipGetLastError());
+        return RT_HIP_OK;
+    }
     // A row is split so that about a thousand workgroups look for the ranges (2048 tokens at least in each) and as many as there are
     // compute units count (4096 tokens at least): every one of the latter adds up to 4096 bins to the row's histogram.  77 rows
     // of 131071: 71 us with 256 workgroups, 73 with 512, 81 with 1024.  Rows go in groups whose histograms stay below 64 MB.

@@ -76,10 +76,12 @@ def test_equal_logits_go_by_index(ex):
     assert check(ex, zeros, 1.0, top_k=3, u=[0.0, 0.4, 0.7, 0.99]).tolist() == [0, 1, 2, 2]
 
 
-def test_infinities_and_nans(ex):
+@pytest.mark.parametrize("pad", [0, 33000])
+def test_infinities_and_nans(ex, pad):
     inf, nan = np.inf, np.nan
     rows = np.array([[0.0, -inf, 1.0, -inf, 2.0], [-inf, -inf, -inf, -inf, -inf], [nan, nan, nan, nan, nan], [nan, 1.0, nan, 2.0, -inf], [inf, 1.0, inf, 2.0, nan],
                      [-3.4e38, 3.4e38, 0.0, 1.0, -inf]])
+    rows = np.pad(rows, ((0, 0), (0, pad)), constant_values=-inf)
     for u in (0.0, 0.3, 0.6, 0.999999):
         for kw in (dict(), dict(top_k=2), dict(top_p=0.5), dict(min_p=0.3), dict(temperature=0.0), dict(top_k=4, top_p=0.9, min_p=0.01), dict(temperature=1e30),
                    dict(temperature=1e-30), dict(temperature=inf)):
@@ -152,23 +154,36 @@ def test_sampling_refuses_what_it_cannot_do(ex):
     ex.synchronize()
 
 
-def test_thousands_of_equal_or_coarse_logits(ex):
+@pytest.mark.parametrize("pad", [0, 40000])          # tokens that cannot be drawn behind the row's: one launch, and four
+def test_thousands_of_equal_or_coarse_logits(ex, pad):
     """More tokens at one value than the device sorts, and logits on the grid that a 16-bit output leaves."""
     rng = np.random.default_rng(11)
     x = np.zeros((6, 5000))
     x[:, 4000:] = -0.5
     x[3:, 777] = 1.0
+    x = np.pad(x, ((0, 0), (0, pad)), constant_values=-np.inf)
     u = [0.0, 0.3, 0.99, 0.01, 0.5, 0.9]
     for kw in (dict(), dict(top_k=2500), dict(top_k=4500, top_p=0.6), dict(top_p=0.99), dict(min_p=0.5), dict(top_k=3, min_p=0.9), dict(top_k=2500, temperature=1e-3)):
         # of 2500 equal tokens 0.3 and 0.99 end exactly behind the 750th and the 2475th: those two rows may go either way
         check(ex, x, u=u, borders=2, **kw)
     coarse = (rng.standard_normal((4, 20000)) * 2).astype(np.float32)
     coarse = (coarse.view(np.uint32) & np.uint32(0xFFFF0000)).view(np.float32)
+    coarse = np.pad(coarse, ((0, 0), (0, pad)), constant_values=-np.inf)
     for kw in (dict(), dict(top_k=50), dict(top_k=3000, top_p=0.7), dict(top_p=0.9), dict(top_p=0.5, min_p=0.2), dict(temperature=8.0, top_p=0.95), dict(temperature=0.05, top_p=0.95)):
         check(ex, coarse, u=rng.random(4), **kw)
 
 
+def test_rows_of_a_large_vocabulary_with_their_own_settings(ex):
+    rng = np.random.default_rng(13)
+    x = rng.standard_normal((24, 50000)) * 2.5
+    check(ex, x, rng.choice([0.0, 0.5, 1.0, 3.0], 24), rng.choice([0, 1, 3, 900, 1024, 1025, 4000, 49999], 24), rng.choice([0.0, 0.3, 0.9, 0.9999], 24),
+          rng.choice([0.0, 0.01, 0.5], 24), rng.random(24))
+
+
 def test_more_rows_than_one_launch_takes(ex):
     rng = np.random.default_rng(12)
+    big = np.full((1100, 33000), -np.inf, dtype=np.float32)      # more rows than the four launches take at a time
+    big[:, ::1100] = rng.standard_normal((1100, 30))
+    check(ex, big, 0.9, rng.integers(0, 12, 1100), rng.choice([0.0, 0.7], 1100), rng.choice([0.0, 0.1], 1100), rng.random(1100))
     x = rng.standard_normal((1500, 40))
     check(ex, x, 0.9, rng.integers(0, 12, 1500), rng.choice([0.0, 0.7], 1500), rng.choice([0.0, 0.1], 1500), rng.random(1500))
