@@ -208,6 +208,11 @@ __device__ __forceinline__ void fold_range(RowRange &g) {
     g.top = top;
     g.low = wave_low(g.low);
 }
+// Orders the LDS traffic of one wave: the hardware runs it in order, the compiler may not move it across this point.
+__device__ __forceinline__ void wave_lds_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
 // A row with nothing to draw from, or nothing to draw: written here.
 __device__ __forceinline__ bool undrawn_row(const SampleArgs &a, int r, const RowAsks &q, const RowRange &g) {
     if (g.top != -INFINITY && !q.greedy) return false;
@@ -446,8 +451,8 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a, 
     const int tid = threadIdx.x, part = blockIdx.x, row = blockIdx.y, r = w.row0 + row;
     const float *x = a.logits + (size_t)r * a.ld;
     const int i0 = part * kPart;
-    float v[kPart / kThreads];
-    load_steps<kPart / kThreads, kThreads>(x + i0, a.vocab - i0, v);      // on their way while the borders are looked for
+    float v[4], next[4];
+    load_steps<4, kThreads>(x + i0, a.vocab - i0, v);      // on their way while the borders are looked for
     const RowAsks q = row_asks(a, r);
     if (q.greedy) return;
     const RowRange g = row_range(w, row);
@@ -467,15 +472,20 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a, 
     const Wanted want(borders);
     const double min_w = ldexp(q.min_w, a.frac_bits);
     unsigned long long mine = 0;
+#pragma unroll 1
+    for (int h = 0; h < kPart; h += 4 * kThreads) {
+        load_steps<4, kThreads>(x + i0 + h + 4 * kThreads, min(a.vocab, i0 + kPart) - i0 - h - 4 * kThreads, next);
 #pragma unroll
-    for (int j = 0; j < kPart / kThreads; j++) {
-        const float at = bin_at(b, v[j]);
-        if (want.kept(at)) {
-            const double f = token_weight(b, v[j]);
-            if (f >= min_w) mine += whole(f);
-        } else if (want.listed(at)) {
-            const int place = __hip_atomic_fetch_add(&n_found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-            if (place < kListMost) found[place] = rank_key(v[j], i0 + tid + j * kThreads);
+        for (int j = 0; j < 4; j++) {
+            const float at = bin_at(b, v[j]);
+            if (want.kept(at)) {
+                const double f = token_weight(b, v[j]);
+                if (f >= min_w) mine += whole(f);
+            } else if (want.listed(at)) {
+                const int place = __hip_atomic_fetch_add(&n_found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+                if (place < kListMost) found[place] = rank_key(v[j], i0 + h + tid + j * kThreads);
+            }
+            v[j] = next[j];
         }
     }
     mine = block_sum_u64(mine, red);                        // its barriers also publish the list
@@ -637,8 +647,11 @@ __device__ __forceinline__ void finish_row(const SampleArgs &a, int r, const Row
                             buf[o] = x0;
                         }
                     }
-                    __syncthreads();
+                    // a wave's exchanges of stride 64 and less lie in 128 keys of its own
+                    if (stride > 64 || (stride == 1 && size > 64)) __syncthreads();
+                    else wave_lds_fence();
                 }
+            __syncthreads();
         }
         unsigned long long run = 0;
 #pragma unroll 1
