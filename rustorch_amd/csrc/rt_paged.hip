@@ -28,6 +28,8 @@ namespace {
 // (i, i + head_dim / 2).  The angle is taken in turns in 64 bits and reduced to [-1/2, 1/2] before it is rounded: at position
 // 100 000 an f32 angle is off by up to 4e-3.  sin and cos of a token's angles are worked out once per workgroup and kept in LDS
 // for all its heads.
+// Bound by memory: 12 bytes of keys and values and 8 of queries per element read and written once.  16 384 ragged tokens of 32 + 8 heads of 128
+// (646 MB): 119 us, 5.4 TB/s (a copy of 4 GiB moves 4.6); one token: 5.2 us, the launch and two dependent reads.
 constexpr int kRopeNone = 0, kRopeInterleaved = 1, kRopeHalf = 2;
 
 struct AppendArgs {
@@ -217,6 +219,7 @@ int rt_hip_paged_append_dev(rt_hip_ctx *ctx, const rt_hip_paged_kv *kv, const in
     if (rc) return rc;
     RT_REQUIRE(ctx, k && v, RT_HIP_ERR_INVALID_ARG, "%s: NULL argument", who);
     RT_REQUIRE(ctx, n_tok >= 0 && (cu_new || n_tok == n_seq), RT_HIP_ERR_SHAPE, "%s: n_tok=%d (without cu_new one token per sequence: %d)", who, n_tok, n_seq);
+    RT_REQUIRE(ctx, n_tok <= 1 << 22, RT_HIP_ERR_SHAPE, "%s: n_tok=%d is beyond one grid", who, n_tok);
     RT_REQUIRE(ctx, rope >= rt::kRopeNone && rope <= rt::kRopeHalf, RT_HIP_ERR_INVALID_ARG, "%s: rope=%d", who, rope);
     RT_REQUIRE(ctx, rope == rt::kRopeNone || (theta > 0.f && theta <= 1e30f), RT_HIP_ERR_INVALID_ARG, "%s: theta=%g", who, (double)theta);
     RT_REQUIRE(ctx, (q != nullptr) == (q_out != nullptr), RT_HIP_ERR_INVALID_ARG, "%s: q and q_out go together", who);

@@ -747,14 +747,9 @@ __global__ __launch_bounds__(64 * W * S, 2) void paged_prefill_kernel(PrefillArg
 namespace {
 template <int HD, int W, int S>
 hipError_t run_prefill(hipStream_t s, const PrefillArgs &a) {
-    auto kernel = paged_prefill_kernel<HD, W, S>;
-    const size_t lds = prefill_lds_bytes<HD, W, S>();
-    if (lds > 64 * 1024) {                                // granted per kernel on request; asking again is harmless, so no state is kept
-        const hipError_t e = hipFuncSetAttribute((const void *)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
-        if (e != hipSuccess) return e;
-    }
     const dim3 grid((unsigned)a.p.n_kv, (unsigned)((long long)a.n_tok * a.group / (32 * W) + a.p.n_seq));
-    kernel<<<grid, 64 * W * S, lds, s>>>(a);
+    const size_t lds = prefill_lds_bytes<HD, W, S>();
+    paged_prefill_kernel<HD, W, S><<<grid, 64 * W * S, lds, s>>>(a);
     return hipGetLastError();
 }
 }  // namespace

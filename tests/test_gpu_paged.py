@@ -424,9 +424,16 @@ def test_paged_calls_refuse_what_they_cannot_do(ex):
         ex.paged_attn_decode_dev(kv, ex.paged_seqs(ints, ints, 4, 4, None, -1), x, 2, x)
     with pytest.raises(InvalidParameters, match="aligned"):
         ex.paged_attn_decode_dev(kv, one, ex.borrow(x.ptr.value + 8, 8192), 2, x)
+    lib = ex.lib
+    big = 1 << 40                                                                # refused by size before anything is looked at
+    for n_tok in ((1 << 22) + 1, -1):
+        assert lib.rt_hip_paged_append_dev(ex.ctx, kv.handle, ints.ptr, 4, ints.ptr, ints.ptr, 4, n_tok, x.ptr, big, x.ptr, big, None, 0, None, 0, 0, 0, 1.0) == 2
+    assert lib.rt_hip_paged_attn_prefill_dev(ex.ctx, kv.handle, ints.ptr, 4, ints.ptr, ints.ptr, 4, 1 << 23, x.ptr, big, 2, x.ptr, big) == 2
+    for n_seq, max_blocks in ((0, 4), (65536, 4), (4, 0), (4, (1 << 26) + 1)):
+        assert lib.rt_hip_paged_attn_decode_dev(ex.ctx, kv.handle, ints.ptr, max_blocks, ints.ptr, n_seq, 0, x.ptr, 128, 2, x.ptr, 128) == 2
+    assert lib.rt_hip_paged_attn_decode_dev(ex.ctx, kv.handle, ints.ptr, 4, ints.ptr, 65535, 0, x.ptr, 8192, 128, x.ptr, 8192) == 2
     ex.paged_append_dev(kv, seqs, x, x, 0)                                       # no tokens: nothing to do
     ex.paged_attn_prefill_dev(kv, seqs, x, 0, 2, x)
-    lib = ex.lib
     assert lib.rt_hip_paged_kv_free(ex.ctx, None) == 0
     assert lib.rt_hip_paged_append_dev(None, None, None, 0, None, None, 0, 0, None, 0, None, 0, None, 0, None, 0, 0, 0, 0.0) == 1
     assert lib.rt_hip_paged_attn_decode_dev(ex.ctx, None, None, 0, None, 0, 0, None, 0, 0, None, 0) == 1
@@ -458,3 +465,30 @@ def test_prefill_attention_of_a_long_prompt(ex, group):
         _, k, v = b.rows(0, h // group, 4 + t)
         want, bound = ref.attention(q[t, h * hd:(h + 1) * hd].astype(np.float64), k, v, hd ** -0.5)
         assert (np.abs(got[t, h * hd:(h + 1) * hd] - want) <= bound).all(), (t, h)
+
+
+def test_two_executors_at_once(ex):
+    """Two contexts, each with a stream and a workspace of its own, run split decode steps over one pool between one another."""
+    from rustorch_amd.executor import HipKernelExecutor
+    rng = np.random.default_rng(40)
+    b = ref.Batch(rng, [3000, 1, 700], 16, 2, 64)
+    d = OnDevice(ex, b)
+    q = [rng.standard_normal((3, 4 * 64)).astype(np.float32) for _ in range(2)]
+    with HipKernelExecutor(0) as other:
+        outs = []
+        for e, x in ((ex, q[0]), (other, q[1])):
+            outs.append((e, e.to_device(x), [e.buffer(x.nbytes) for _ in range(4)]))
+        pools = [e.wrap_paged_kv(d.k, d.v, b.n_pages, 16, 2, 64) for e, _, _ in outs]
+        for i in range(4):
+            for (e, dq, out), pool in zip(outs, pools):
+                e.paged_attn_decode_dev(pool, d.seqs, dq, 4, out[i])
+        for (e, _, out), x in zip(outs, q):
+            got = [o.download(np.float32) for o in out]
+            assert all(np.array_equal(got[0], g) for g in got)               # the same bits every time
+            for s in range(3):
+                for h in range(4):
+                    _, k, v = b.rows(s, h // 2, int(b.kv_len[s]))
+                    want, bound = ref.attention(x[s, h * 64:(h + 1) * 64].astype(np.float64), k, v, 1 / 8)
+                    assert (np.abs(got[0].reshape(3, 4, 64)[s, h] - want) <= bound).all()
+        for p in pools:
+            p.free()
