@@ -254,7 +254,9 @@ RT_HIP_API int rt_hip_argmax_dev(rt_hip_ctx *ctx, const float *v, size_t n, int 
  *                                         last positions; ascending
  *      What they say is checked where it is used: a page id outside the pool is never followed (its positions are not stored
  *      and not seen), a length beyond max_blocks * page_size counts as that, a row that no sequence owns is left as it was.
- *      Sequences may share pages that are only read.  Rows of q, k, v and the outputs are *_ld floats apart (a multiple of 4, at
+ *      Sequences may share pages that are only read.  A call takes up to 65535 sequences of up to 2^30 positions, append up to 2^22
+ *      tokens, decode up to 2^22 rows times query heads, prefill up to 65535 * 64 rows of tokens times query heads per key / value
+ *      head.  Rows of q, k, v and the outputs are *_ld floats apart (a multiple of 4, at
  *      least the row's length), their bases 16-byte aligned; query head h reads key / value head h / (n_heads / n_kv_heads). */
 RT_HIP_API int rt_hip_paged_kv_create(rt_hip_ctx *ctx, size_t n_pages, int page_size, int n_kv_heads, int head_dim, rt_hip_paged_kv **out);
 RT_HIP_API int rt_hip_paged_kv_wrap_dev(rt_hip_ctx *ctx, uint16_t *k_pages, uint16_t *v_pages, size_t n_pages, int page_size, int n_kv_heads,

@@ -28,7 +28,7 @@ namespace {
 // (i, i + head_dim / 2).  The angle is taken in turns in 64 bits and reduced to [-1/2, 1/2] before it is rounded: at position
 // 100 000 an f32 angle is off by up to 4e-3.  sin and cos of a token's angles are worked out once per workgroup and kept in LDS
 // for all its heads.
-// Bound by memory: 12 bytes of keys and values and 8 of queries per element read and written once.  16 384 ragged tokens of 32 + 8 heads of 128
+// Bound by memory: 12 bytes of keys and values and 8 of queries per element read and written once.  14 334 ragged tokens of 32 + 8 heads of 128
 // (646 MB): 119 us, 5.4 TB/s (a copy of 4 GiB moves 4.6); one token: 5.2 us, the launch and two dependent reads.
 constexpr int kRopeNone = 0, kRopeInterleaved = 1, kRopeHalf = 2;
 

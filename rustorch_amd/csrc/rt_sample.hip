@@ -129,7 +129,8 @@ struct SampleWork {
     int *listed;                                           // [row]: tokens listed
     unsigned long long *list;                              // [row][kListMost]: their keys
     unsigned long long *part_sum;                          // [row][part]: weight that stays whole, of kPart tokens each
-    int row0, splits, per_split, per_count, parts;                    // this launch's first row
+    int row0;                                              // this launch's first row
+    int splits, per_split, per_count, parts, parts_each;
 };
 
 struct RowBins {
@@ -443,16 +444,18 @@ struct Wanted {
     __device__ bool listed(float at) const { return (at >= p0 && at < p1) || (at >= k0 && at < k1); }
 };
 
-// One workgroup per kPart tokens of a row: lists the tokens of the cuts' bins and sums the weights of the tokens above them.
+// Lists the tokens of the cuts' bins and sums the weights of the tokens above them, kPart tokens at a time; a workgroup has
+// parts_each such parts of a row.  Finding the borders takes a workgroup longer than a part does: 77 rows of 131071 with top-k 40 and
+// top-p 0.95 take 59.5 us in all with one part each, 49.8 us with two (1024 workgroups), 51.5 with four, 61.5 with nine.
 __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a, SampleWork w) {
     __shared__ unsigned long long found[kListMost], red[kThreads / 64];
     __shared__ RowBorders borders;
     __shared__ int n_found, place;
-    const int tid = threadIdx.x, part = blockIdx.x, row = blockIdx.y, r = w.row0 + row;
-    const float *x = a.logits + (size_t)r * a.ld;
-    const int i0 = part * kPart;
-    float v[4], next[4];
-    load_steps<4, kThreads>(x + i0, a.vocab - i0, v);      // on their way while the borders are looked for
+    const int tid = threadIdx.x, row = blockIdx.y, r = w.row0 + row, first = (int)blockIdx.x * w.parts_each, last = min(w.parts, first + w.parts_each);
+    const float *x = a.logits + (size_t)r * a.ld + (size_t)first * kPart;
+    const int n_tokens = min(a.vocab, last * kPart) - first * kPart;
+    float v[8], next[8];
+    load_steps<8, kThreads>(x, n_tokens, v);                // on their way while the borders are looked for
     const RowAsks q = row_asks(a, r);
     if (q.greedy) return;
     const RowRange g = row_range(w, row);
@@ -468,31 +471,33 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a, 
         }
     }
     __syncthreads();
-    if (part == 0 && tid == 0) w.borders[row] = borders;
+    if (first == 0 && tid == 0) w.borders[row] = borders;
     const Wanted want(borders);
     const double min_w = ldexp(q.min_w, a.frac_bits);
     unsigned long long mine = 0;
 #pragma unroll 1
-    for (int h = 0; h < kPart; h += 4 * kThreads) {
-        load_steps<4, kThreads>(x + i0 + h + 4 * kThreads, min(a.vocab, i0 + kPart) - i0 - h - 4 * kThreads, next);
+    for (int h = 0; h < n_tokens; h += 8 * kThreads) {
+        load_steps<8, kThreads>(x + h + 8 * kThreads, n_tokens - h - 8 * kThreads, next);
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < 8; j++) {
             const float at = bin_at(b, v[j]);
             if (want.kept(at)) {
                 const double f = token_weight(b, v[j]);
                 if (f >= min_w) mine += whole(f);
             } else if (want.listed(at)) {
                 const int place = __hip_atomic_fetch_add(&n_found, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-                if (place < kListMost) found[place] = rank_key(v[j], i0 + h + tid + j * kThreads);
+                if (place < kListMost) found[place] = rank_key(v[j], first * kPart + h + tid + j * kThreads);
             }
             v[j] = next[j];
         }
+        if ((h / (8 * kThreads)) % (kPart / (8 * kThreads)) == kPart / (8 * kThreads) - 1 || h + 8 * kThreads >= n_tokens) {      // the end of a part
+            mine = want.keep > 0.f ? block_sum_u64(mine, red) : 0;
+            if (tid == 0) w.part_sum[(size_t)row * w.parts + first + h / kPart] = mine;
+            mine = 0;
+        }
     }
-    mine = block_sum_u64(mine, red);                        // its barriers also publish the list
-    if (tid == 0) {
-        w.part_sum[(size_t)row * w.parts + part] = mine;
-        place = n_found ? __hip_atomic_fetch_add(&w.listed[row], n_found, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
-    }
+    __syncthreads();
+    if (tid == 0) place = n_found ? __hip_atomic_fetch_add(&w.listed[row], n_found, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) : 0;
     __syncthreads();
     const int at = place, n = min(n_found, kListMost);      // more than the list holds: the count says so
     for (int i = tid; i < n; i += kThreads)
@@ -896,7 +901,7 @@ int rt_hip_sample_dev(rt_hip_ctx *ctx, const float *logits, size_t ld, int n_row
     // One workgroup per row, or rows split over the device in four launches (us; top-k 40 and top-p 0.95 / top-p 0.9 / no filter):
     //   rows x vocab    1 x 32000   64 x 32000  256 x 32000  64 x 65536  77 x 131071  1 x 131071
     //   one launch      23/42/23    24/44/24    28/47/27     34/73/39    59/135/73    50/127/65
-    //   four            26/31/21    40/55/27    55/78/42     46/63/31    62/94/44     30/36/20
+    //   four            26/31/21    40/55/27    55/78/42     39/53/30    50/78/43     30/36/20
     if (vocab <= 32768) {
         rt::sample_row_kernel<<<dim3((unsigned)n_rows), rt::kRowThreads, 0, ctx->stream>>>(a);
         RT_TRY_HIP(ctx, hipGetLastError());
@@ -912,6 +917,7 @@ int rt_hip_sample_dev(rt_hip_ctx *ctx, const float *logits, size_t ld, int n_row
     w.per_split = (vocab + w.splits - 1) / w.splits;
     w.per_count = (vocab + count_splits - 1) / count_splits;
     w.parts = (vocab + rt::kPart - 1) / rt::kPart;
+    w.parts_each = std::max(1, std::min(w.parts, w.parts * group / 1024));
     const size_t coarse = (size_t)group * rt::kCoarse, bins = (size_t)group * rt::kBins, list = (size_t)group * rt::kListMost, parts = (size_t)group * w.parts;
     int rc = ensure_scratch(ctx, (bins + list + parts + coarse) * 8 + group * sizeof(rt::RowBorders) + (size_t)group * w.splits * sizeof(rt::RowRange) +
                                  (bins + coarse + group) * 4);
@@ -930,7 +936,7 @@ int rt_hip_sample_dev(rt_hip_ctx *ctx, const float *logits, size_t ld, int n_row
         const dim3 grid((unsigned)w.splits, (unsigned)rows);
         rt::sample_range_kernel<<<grid, rt::kThreads, 0, ctx->stream>>>(a, w);
         rt::sample_histogram_kernel<<<dim3((unsigned)count_splits, (unsigned)rows), rt::kCountThreads, 0, ctx->stream>>>(a, w);
-        rt::sample_collect_kernel<<<dim3((unsigned)w.parts, (unsigned)rows), rt::kThreads, 0, ctx->stream>>>(a, w);
+        rt::sample_collect_kernel<<<dim3((unsigned)((w.parts + w.parts_each - 1) / w.parts_each), (unsigned)rows), rt::kThreads, 0, ctx->stream>>>(a, w);
         rt::sample_finish_kernel<<<dim3((unsigned)rows), rt::kThreads, 0, ctx->stream>>>(a, w);
     }
     RT_TRY_HIP(ctx, hipGetLastError());
