@@ -55,7 +55,6 @@ __device__ __forceinline__ int units_of(int len) { return (len + kChunkUnit - 1)
 // Units per chunk: whole waves call this, every wave of the grid gets the same answer.  sum(units) / budget, rounded up past
 // the sum's own rounding, so that sum over sequences of ceil(units / chunk) <= budget + n_seq.
 __device__ __forceinline__ int chunk_units(const PagedView &p, int budget) {
-    if (budget == 0) return 1 << 30;
     float total = 0.f;
     for (int s0 = 0; s0 < p.n_seq; s0 += 64) total += (float)units_of(length_of(p, s0 + (int)(threadIdx.x & 63)));
     total = wave_sum(total);
@@ -77,26 +76,31 @@ __global__ __launch_bounds__(64 * kDecodeWaves, OCC) void paged_decode_kernel(De
     const bool has_head = head_in_group < a.group;
 
     // ---- which chunk of which sequence
-    const int per_chunk = chunk_units(p, a.budget);
-    int seq = -1, nth = 0, chunks = 1, len = 0;
-    for (int s0 = 0, before = 0; s0 < p.n_seq; s0 += 64) {
-        const int its = length_of(p, s0 + lane), mine = s0 + lane < p.n_seq ? chunks_of(units_of(its), per_chunk) : 0;
-        int upto = mine;                     // running sum over the lanes
+    int seq = -1, nth = 0, chunks = 1, len = 0, per_chunk = 0;
+    if (a.budget == 0) {
+        seq = unit;
+        len = length_of(p, seq);
+    } else {
+        per_chunk = chunk_units(p, a.budget);
+        for (int s0 = 0, before = 0; s0 < p.n_seq; s0 += 64) {
+            const int its = length_of(p, s0 + lane), mine = s0 + lane < p.n_seq ? chunks_of(units_of(its), per_chunk) : 0;
+            int upto = mine;                     // running sum over the lanes
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int below = __shfl_up(upto, o);
-            if (lane >= o) upto += below;
+            for (int o = 1; o < 64; o <<= 1) {
+                const int below = __shfl_up(upto, o);
+                if (lane >= o) upto += below;
+            }
+            const unsigned long long past = __ballot(before + upto > unit);
+            if (past) {
+                const int l = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
+                seq = s0 + l;
+                chunks = __builtin_amdgcn_readlane(mine, l);
+                len = __builtin_amdgcn_readlane(its, l);
+                nth = unit - before - (__builtin_amdgcn_readlane(upto, l) - chunks);
+                break;
+            }
+            before += __builtin_amdgcn_readlane(upto, 63);
         }
-        const unsigned long long past = __ballot(before + upto > unit);
-        if (past) {
-            const int l = __builtin_amdgcn_readfirstlane(__ffsll(past) - 1);
-            seq = s0 + l;
-            chunks = __builtin_amdgcn_readlane(mine, l);
-            len = __builtin_amdgcn_readlane(its, l);
-            nth = unit - before - (__builtin_amdgcn_readlane(upto, l) - chunks);
-            break;
-        }
-        before += __builtin_amdgcn_readlane(upto, 63);
     }
     if (seq < 0) return;                     // the grid is cut for the most chunks there may be
     if (a.budget > 0 && nth == 0 && hx == 0 && threadIdx.x == 0) a.plan[seq] = make_int2(unit, chunks);
@@ -403,7 +407,7 @@ namespace {
 // An infinite or NaN value at a position that some of a tile's rows do not see would enter their sums as 0 * inf.  Tiles that
 // reach beyond a row are looked through for such values; a workgroup that meets one does its rows again, one at a time.
 // Measured: one prompt of 8191 tokens, 32 heads over 8 kv heads of 128: 1.05 ms = 524 TFLOP/s of the formula, 1048 of fp16 products (a
-// library product of 8192^3 reaches 1139); a prompt of 512, 32 kv heads: 22 us.
+// library product of 8192^3 reaches 1139); a prompt of 512, 32 kv heads: 21.8 us.
 constexpr int kPrefillKeys = 32;
 
 struct PrefillArgs {
@@ -669,23 +673,26 @@ __global__ __launch_bounds__(64 * W * S, 2) void paged_prefill_kernel(PrefillArg
                 phi[r >> 3][r & 7] = hi[0]; phi[r >> 3][(r & 7) + 1] = hi[1];
                 plo[r >> 3][r & 7] = lo[0]; plo[r >> 3][(r & 7) + 1] = lo[1];
             }
-            // slot e of product mm stands for row 16 mm + 8 (e / 4) + 4 hh + e % 4 of the tile
+            // slot e of product mm stands for row 16 mm + 8 (e / 4) + 4 hh + e % 4 of the tile; the products of one block of dims wait for
+            // one another, so the blocks take turns
 #pragma unroll
-            for (int db = 0; db < DB; db++)
+            for (int mm = 0; mm < 2; mm++) {
+                half8v av[DB];
 #pragma unroll
-                for (int mm = 0; mm < 2; mm++) {
-                    half8v av;
+                for (int db = 0; db < DB; db++)
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
                         const int row = 16 * mm + 8 * h + vrow0, col = 32 * db + vcol0, ch = col >> 3;
                         const int vc = HD == 128 ? ch ^ (4 * (row & 3)) : ch ^ (4 * ((row >> 1) & 1));
                         const half4v x = read_transposed(vs + buf * KT * HD + row * HD + 8 * vc + (col & 7));
 #pragma unroll
-                        for (int e = 0; e < 4; e++) av[4 * h + e] = x[e];
+                        for (int e = 0; e < 4; e++) av[db][4 * h + e] = x[e];
                     }
-                    acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, phi[mm], acc[db], 0, 0, 0);
-                    acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av, plo[mm], acc[db], 0, 0, 0);
-                }
+#pragma unroll
+                for (int db = 0; db < DB; db++) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av[db], phi[mm], acc[db], 0, 0, 0);
+#pragma unroll
+                for (int db = 0; db < DB; db++) acc[db] = __builtin_amdgcn_mfma_f32_32x32x16_f16(av[db], plo[mm], acc[db], 0, 0, 0);
+            }
         }
         if (n + 1 < steps) {
             put(min(t + S, tiles - 1), buf ^ 1, ok_next);
@@ -759,8 +766,8 @@ hipError_t launch_paged_prefill(hipStream_t s, const PagedView &p, int head_dim,
     // 128 rows a workgroup and two of those per compute unit read the keys least often; with fewer than two and a half such workgroups
     // per compute unit, 64 rows and two groups of waves that share the positions end sooner (32 heads of 128, one prompt; us):
     //   tokens          64   256   512  1024  2048  3000  4096  6000
-    //   128 rows       9.0  19.9  31.9  54.8   108   180   320   644
-    //   64 rows, two   9.5  14.9  22.3  38.6   101   198   347   726
+    //   128 rows       9.0  19.9  31.9  54.8   108   179   317   630
+    //   64 rows, two   9.4  14.7  21.8  38.1   101   198   347   726
     // Heads of 64 take half the registers and LDS, and the smaller form throughout (16 heads, 6000 tokens: 205 for 220 us).
     if (head_dim == 64) return run_prefill<64, 2, 2>(s, a);
     if ((long long)n_tok * a.group / 128 * p.n_kv >= 640) return run_prefill<128, 4, 1>(s, a);
