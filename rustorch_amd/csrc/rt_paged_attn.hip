@@ -108,6 +108,18 @@ __global__ __launch_bounds__(64 * kDecodeWaves, OCC) void paged_decode_kernel(De
     const int n = chunks == 1 ? len : min(per_chunk * kChunkUnit, len - first);      // positions of this chunk (0: an empty sequence)
     const int tiles = (n + kTileKeys - 1) / kTileKeys;
 
+    // ---- the chunk's pages, 64 table entries at a time: one per lane, bad ids as -1 (asked for before the queries are
+    // split: the first tile waits for it; 33 sequences of 1 to 4097 positions 63.1 for 63.5 us)
+    const int page0 = (int)(first >> p.page_shift);
+    int window = 0, entry = -1;                               // entry of lane l: table[page0 + 64 * window + l]
+    auto load_window = [&](int w) {
+        const int i = page0 + 64 * w + lane;
+        int id = i < p.max_blocks ? p.table[(size_t)seq * p.max_blocks + i] : -1;
+        entry = id >= 0 && id < p.n_pages ? id : -1;
+        window = w;
+    };
+    if (n > 0) load_window(0);
+
     // ---- the queries: lane (g, c) holds dims 32 kk + 8 g .. + 7 of head c, split in two halves
     half8v qhi[KK], qlo[KK];
     float sscale;
@@ -140,17 +152,6 @@ __global__ __launch_bounds__(64 * kDecodeWaves, OCC) void paged_decode_kernel(De
                 qlo[kk][e] = (_Float16)(v - (float)hi);
             }
     }
-
-    // ---- the chunk's pages, 64 table entries at a time: one per lane, bad ids as -1
-    const int page0 = (int)(first >> p.page_shift);
-    int window = 0, entry = -1;                               // entry of lane l: table[page0 + 64 * window + l]
-    auto load_window = [&](int w) {
-        const int i = page0 + 64 * w + lane;
-        int id = i < p.max_blocks ? p.table[(size_t)seq * p.max_blocks + i] : -1;
-        entry = id >= 0 && id < p.n_pages ? id : -1;
-        window = w;
-    };
-    if (n > 0) load_window(0);
 
     // ---- a tile: G groups of 16 consecutive positions, each inside one page
     const size_t k_lane = (size_t)c * HD + 8 * g, v_lane = (size_t)(4 * g) * HD + VE * c;
