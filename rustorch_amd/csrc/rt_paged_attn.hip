@@ -8,7 +8,6 @@
 namespace rt {
 namespace {
 
-typedef _Float16 half8v __attribute__((ext_vector_type(8)));
 typedef float float4v __attribute__((ext_vector_type(4)));
 
 // ------------------------------------------------------------------------------------------- one query per sequence
@@ -16,8 +15,8 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 // the loads, for one query head per kv head as well as for sixteen.  Both products run on the matrix cores in shapes whose
 // operands are what a lane loads, with no exchange between lanes:
 //   S[key][head] = K . Q^T      v_mfma_f32_16x16x32_f16: lane (g = l / 16, c = l % 16) loads 16 bytes of key c; Q is split into
-//                               two halves (value = hi + lo, after a power-of-two scaling), f32 accuracy for two instructions;
-//                               the lane ends with the scores of head c and keys 4 g + r, r < 4
+//                               two halves (split_query), f32 accuracy for two instructions; the lane ends with the scores of
+//                               head c and keys 4 g + r, r < 4
 //   O^T[dim][head] = V^T . P    v_mfma_f32_16x16x4_f32, k = g: the lane's register p_r is the second operand as it stands if the
 //                               first is the value row 4 g + r, of which the lane loads chunk c: element e of the chunk is
 //                               dim VE c + e, so there is one accumulator per e
@@ -124,7 +123,7 @@ __global__ __launch_bounds__(64 * kDecodeWaves, OCC) void paged_decode_kernel(De
     half8v qhi[KK], qlo[KK];
     float sscale;
     {
-        float qf[KK][8], amax = 0.f;
+        float qf[KK][8], amax = 0.f, amin = INFINITY;
         const float *qp = a.q + (size_t)seq * a.q_ld + (size_t)(has_head ? head : kvh * a.group) * HD + 8 * g;
 #pragma unroll
         for (int kk = 0; kk < KK; kk++) {
@@ -132,7 +131,10 @@ __global__ __launch_bounds__(64 * kDecodeWaves, OCC) void paged_decode_kernel(De
             qf[kk][0] = x.x; qf[kk][1] = x.y; qf[kk][2] = x.z; qf[kk][3] = x.w;
             qf[kk][4] = y.x; qf[kk][5] = y.y; qf[kk][6] = y.z; qf[kk][7] = y.w;
 #pragma unroll
-            for (int e = 0; e < 8; e++) amax = fmaxf(amax, fabsf(qf[kk][e]));
+            for (int e = 0; e < 8; e++) {
+                amax = fmaxf(amax, fabsf(qf[kk][e]));
+                amin = fminf(amin, fabsf(qf[kk][e]));
+            }
         }
         amax = fmaxf(amax, __shfl_xor(amax, 16));
         amax = fmaxf(amax, __shfl_xor(amax, 32));
@@ -142,15 +144,20 @@ __global__ __launch_bounds__(64 * kDecodeWaves, OCC) void paged_decode_kernel(De
         const float qscale = ldexpf(1.0f, 14 - ex);
         // scores in units of log2: exp2 is the hardware's own exponential
         sscale = ldexpf(1.0f, ex - 14) * (1.44269504088896341f / sqrtf((float)HD));
+        if (__ballot(!(amin * qscale >= 0x1p-24f)) == 0) {
 #pragma unroll
-        for (int kk = 0; kk < KK; kk++)
+            for (int kk = 0; kk < KK; kk++) split_queries(qf[kk], qscale, qhi[kk], qlo[kk]);
+        } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float v = qf[kk][e] * qscale;
-                const _Float16 hi = (_Float16)v;
-                qhi[kk][e] = hi;
-                qlo[kk][e] = (_Float16)(v - (float)hi);
-            }
+            for (int kk = 0; kk < KK; kk++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    _Float16 hi, lo;
+                    split_query(qf[kk][e], qscale, hi, lo);
+                    qhi[kk][e] = hi;
+                    qlo[kk][e] = lo;
+                }
+        }
     }
 
     // ---- a tile: G groups of 16 consecutive positions, each inside one page
@@ -396,8 +403,8 @@ namespace {
 // Bound by the matrix cores.  The rows of one kv head of one sequence -- its new tokens times the query heads that share the kv
 // head -- are packed one after the other; a wave has 32 of them, a workgroup 32 W, and the workgroup's keys and values go through
 // LDS once for all of them.  Flash style, tiles of 32 positions:
-//   S^T[key][row]  = K . (Qhi + Qlo)^T    v_mfma_f32_32x32x16_f16, the f32 side in two halves (value = hi + lo after a power-of-two
-//                                         scaling): f32 accuracy for twice the products.  A lane's 16 scores belong to one row.
+//   S^T[key][row]  = K . (Qhi + Qlo)^T    v_mfma_f32_32x32x16_f16, the f32 side in two halves (split_query): f32 accuracy for twice
+//                                         the products.  A lane's 16 scores belong to one row.
 //   O^T[dim][row]  = V^T . (Phi + Plo)^T  a lane's 16 probabilities are, as they stand, the second operand; the first wants four
 //                                         consecutive keys of one dim per register pair, which ds_read_b64_tr_b16 reads from the
 //                                         row-major tile.
@@ -534,10 +541,20 @@ __global__ __launch_bounds__(64 * W * S, 2) void paged_prefill_kernel(PrefillArg
     half8v qhi[KK], qlo[KK];
     float sscale;
     {
-        float amax = 0.f;
-        for (int kk = 0; kk < KK; kk++) {
+        float amax = 0.f, amin = INFINITY;
+        auto eight = [&](int kk, float (&f)[8]) {
             const float4 x = *reinterpret_cast<const float4 *>(qrow + 16 * kk + 8 * hh), y = *reinterpret_cast<const float4 *>(qrow + 16 * kk + 8 * hh + 4);
-            amax = fmaxf(amax, fmaxf(fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w))), fmaxf(fmaxf(fabsf(y.x), fabsf(y.y)), fmaxf(fabsf(y.z), fabsf(y.w)))));
+            f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w;
+            f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
+        };
+        for (int kk = 0; kk < KK; kk++) {
+            float f[8];
+            eight(kk, f);
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                amax = fmaxf(amax, fabsf(f[e]));
+                amin = fminf(amin, fabsf(f[e]));
+            }
         }
         amax = fmaxf(amax, __shfl_xor(amax, 32));
         int ex = 0;
@@ -545,16 +562,25 @@ __global__ __launch_bounds__(64 * W * S, 2) void paged_prefill_kernel(PrefillArg
         ex = max(ex, -100);
         const float qscale = ldexpf(1.0f, 14 - ex);
         sscale = ldexpf(1.0f, ex - 14) * (1.44269504088896341f / sqrtf((float)HD));       // scores in units of log2
+        if (__ballot(!(amin * qscale >= 0x1p-24f)) == 0) {
 #pragma unroll
-        for (int kk = 0; kk < KK; kk++) {
-            const float4 x = *reinterpret_cast<const float4 *>(qrow + 16 * kk + 8 * hh), y = *reinterpret_cast<const float4 *>(qrow + 16 * kk + 8 * hh + 4);
-            const float f[8] = { x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w };
+            for (int kk = 0; kk < KK; kk++) {
+                float f[8];
+                eight(kk, f);
+                split_queries(f, qscale, qhi[kk], qlo[kk]);
+            }
+        } else {
 #pragma unroll
-            for (int e = 0; e < 8; e++) {
-                const float v = f[e] * qscale;
-                const _Float16 hi = (_Float16)v;
-                qhi[kk][e] = hi;
-                qlo[kk][e] = (_Float16)(v - (float)hi);
+            for (int kk = 0; kk < KK; kk++) {
+                float f[8];
+                eight(kk, f);
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    _Float16 hi, lo;
+                    split_query(f[e], qscale, hi, lo);
+                    qhi[kk][e] = hi;
+                    qlo[kk][e] = lo;
+                }
             }
         }
     }
