@@ -455,12 +455,13 @@ __device__ void attend_row(const PagedView &p, const float *q, float *out, int s
         for (int e = 0; e < E; e++) s += qv[e] * h2f(p.k[at + e]);
         s = wave_sum(s);
         const float m_new = fmaxf(m, s);
-        const float keep = m_new == -INFINITY ? 1.f : expf(m - m_new), w = m_new == -INFINITY ? 0.f : expf(s - m_new);
+        const float keep = m_new == -INFINITY ? 1.f : expf(m - m_new), w = s == -INFINITY ? 0.f : expf(s - m_new);      // a score of NaN: NaN
         l = l * keep + w;
         for (int e = 0; e < E; e++) acc[e] = acc[e] * keep + w * h2f(p.v[at + e]);
         m = m_new;
     }
-    for (int e = 0; e < E; e++) out[E * lane + e] = l == 0.f ? 0.f : acc[e] / l;
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    for (int e = 0; e < E; e++) out[E * lane + e] = acc[e] * inv;
 }
 
 // W waves of 32 rows, and S such groups of waves that take the tiles in turn, each with running states and LDS tiles of its own; they

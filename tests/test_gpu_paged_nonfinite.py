@@ -120,3 +120,21 @@ def test_attention_over_keys_that_all_score_minus_infinity(ex):
     q = np.abs(rng.standard_normal((10, 64))).astype(np.float32) + np.float32(0.01)
     assert (prefill(ex, b, q, 1) == 0).all()
     assert (decode(ex, b, q[:2].copy(), 1) == 0).all()
+
+
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+def test_prefill_attention_with_a_bad_first_key_and_a_later_bad_value(ex, bad):
+    """A key that is no number at the first position makes every row NaN, also a row that is done again by itself because a value
+    behind it is not finite; a score of -inf there weighs nothing, and 0 times an infinity is NaN also for a row of no weight."""
+    rng = np.random.default_rng(4)
+    b = ref.Batch(rng, [30, 30], 16, 1, 64, [30, 30])
+    pg, sl = place(b, 0, 0)
+    b.k[pg, 0, sl] = np.nan if np.isnan(bad) else b.k[pg, 0, sl]
+    b.k[pg, 0, sl, 3] = bad
+    pg, sl = place(b, 0, 20)
+    b.v[pg, 0, sl, 9] = np.inf
+    b.k[b.table[1, :2], 0, :, 5] = bad                           # sequence 1: every key
+    b.v[b.table[1, 0], 0, 4, 2] = np.inf
+    b.v[b.table[1, 1], 0, 4, 1] = np.nan
+    got = prefill(ex, b, queries(rng, "f32", 60, 2 * 64), 2)
+    assert np.isnan(got[:30]).any()
