@@ -282,7 +282,10 @@ RT_HIP_API int rt_hip_paged_append_dev(rt_hip_ctx *ctx, const rt_hip_paged_kv *k
 RT_HIP_API int rt_hip_paged_attn_decode_dev(rt_hip_ctx *ctx, const rt_hip_paged_kv *kv, const int *block_table, int max_blocks, const int *kv_len,
                                             int n_seq, int max_kv_len, const float *q, size_t q_ld, int n_heads, float *out, size_t out_ld);
 /* The new tokens of every sequence at once: row cu_new[s] + i (position kv_len[s] - (cu_new[s + 1] - cu_new[s]) + i) over the
- * positions up to its own. */
+ * positions up to its own.
+ * Both attentions keep to the formula where keys or values are not finite (an append stores a key above 65504 as infinity): a
+ * position that scores -inf weighs nothing, a score of +inf or NaN makes the row NaN, an infinite value that is seen comes out as
+ * that infinity in its dim, and what a row does not see never reaches it.  Weights are f32: one below 2^-149 of the largest is 0. */
 RT_HIP_API int rt_hip_paged_attn_prefill_dev(rt_hip_ctx *ctx, const rt_hip_paged_kv *kv, const int *block_table, int max_blocks, const int *kv_len,
                                              const int *cu_new, int n_seq, int n_tok, const float *q, size_t q_ld, int n_heads, float *out,
                                              size_t out_ld);

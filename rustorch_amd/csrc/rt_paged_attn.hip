@@ -412,8 +412,10 @@ namespace {
 // while the current one is used, the one behind it is requested then: one barrier per tile.
 // The grid runs kv heads first: neighbouring workgroups land on different XCDs, so an XCD sees few kv heads and keeps their keys and
 // values in its L2; later rows, which have more keys, go first.
-// An infinite or NaN value at a position that some of a tile's rows do not see would enter their sums as 0 * inf.  Tiles that
-// reach beyond a row are looked through for such values; a workgroup that meets one does its rows again, one at a time.
+// A value that is not finite makes NaN of a row's sums where it should not: at a position that the row does not see, as 0 * inf, and
+// at one that it sees, where a half of the probability is zero.  Rows whose outputs are NaN at the end though their weights are not
+// are done again by themselves (attend_row), where a value meets its weight once and only if it is seen: nothing in the loop
+// over the tiles looks for such values.  A weight that f32 cannot hold (below 2^-149 of the largest) is zero there too, and NaN with them.
 // Measured: one prompt of 8191 tokens, 32 heads over 8 kv heads of 128: 1.05 ms = 524 TFLOP/s of the formula, 1048 of fp16 products (a
 // library product of 8192^3 reaches 1139); a prompt of 512, 32 kv heads: 21.8 us.
 constexpr int kPrefillKeys = 32;
@@ -436,28 +438,43 @@ typedef _Float16 half2v __attribute__((ext_vector_type(2)));
 typedef float float16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 
-// One row of one query head by one wave, the positions one after the other: nothing that is not seen is touched.
+// One row of one query head by one wave: nothing that is not seen is touched, and a value meets its weight once.  64 positions at a time,
+// a lane scoring one of them, then their values one after the other.
 template <int HD>
 __device__ void attend_row(const PagedView &p, const float *q, float *out, int seq, int kvh, int n) {
-    constexpr int E = HD / 64;               // elements of the head a lane holds
+    constexpr int E = HD / 64;               // elements of the output that a lane holds
     const int lane = (int)(threadIdx.x & 63);
     const float scale = 1.0f / sqrtf((float)HD);
-    float qv[E], acc[E], m = -INFINITY, l = 0.f;
-    for (int e = 0; e < E; e++) {
-        qv[e] = q[E * lane + e] * scale;
-        acc[e] = 0.f;
-    }
-    for (int j = 0; j < n; j++) {
-        const int page = p.table[(size_t)seq * p.max_blocks + (j >> p.page_shift)];
-        if (page < 0 || page >= p.n_pages) continue;
-        const size_t at = ((((size_t)page * p.n_kv + kvh) << p.page_shift) + (size_t)(j & ((1 << p.page_shift) - 1))) * HD + E * lane;
+    float acc[E], m = -INFINITY, l = 0.f;
+    for (int e = 0; e < E; e++) acc[e] = 0.f;
+    for (int j0 = 0; j0 < n; j0 += 64) {
+        const int j = j0 + lane, page = j < n ? p.table[(size_t)seq * p.max_blocks + (j >> p.page_shift)] : -1;
+        const bool seen = page >= 0 && page < p.n_pages;
+        const size_t at = ((((size_t)(seen ? page : 0) * p.n_kv + kvh) << p.page_shift) + (size_t)(j & ((1 << p.page_shift) - 1))) * HD;
         float s = 0.f;
-        for (int e = 0; e < E; e++) s += qv[e] * h2f(p.k[at + e]);
-        s = wave_sum(s);
-        const float m_new = fmaxf(m, s);
+#pragma unroll 4
+        for (int d = 0; d < HD; d += 8) {
+            const half8v k = *reinterpret_cast<const half8v *>(p.k + at + d);
+            const float4 x = *reinterpret_cast<const float4 *>(q + d), y = *reinterpret_cast<const float4 *>(q + d + 4);
+            s += ((x.x * (float)k[0] + x.y * (float)k[1]) + (x.z * (float)k[2] + x.w * (float)k[3])) +
+                 ((y.x * (float)k[4] + y.y * (float)k[5]) + (y.z * (float)k[6] + y.w * (float)k[7]));
+        }
+        s = seen ? s * scale : -INFINITY;
+        const float m_new = fmaxf(m, wave_max(s));
         const float keep = m_new == -INFINITY ? 1.f : expf(m - m_new), w = s == -INFINITY ? 0.f : expf(s - m_new);      // a score of NaN: NaN
-        l = l * keep + w;
-        for (int e = 0; e < E; e++) acc[e] = acc[e] * keep + w * h2f(p.v[at + e]);
+        l = l * keep + wave_sum(w);
+        for (int e = 0; e < E; e++) acc[e] *= keep;
+        const int here = min(64, n - j0);
+#pragma unroll 4
+        for (int i = 0; i < here; i++) {
+            const size_t row = ((size_t)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(at >> 32), i) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)at, i);
+            const float weight = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), i));
+            const bool is = __builtin_amdgcn_readlane(seen ? 1 : 0, i) != 0;
+            for (int e = 0; e < E; e++) {
+                const float v = h2f(p.v[row + E * lane + e]);
+                acc[e] += weight * (is ? v : 0.f);
+            }
+        }
         m = m_new;
     }
     const float inv = l == 0.f ? 0.f : 1.0f / l;
@@ -477,7 +494,6 @@ __global__ __launch_bounds__(64 * W * S, 2) void paged_prefill_kernel(PrefillArg
     static_assert(NL >= 1 && (16 % ROWS_AT_ONCE == 0 || ROWS_AT_ONCE % 16 == 0), "a load covers whole groups of 16 positions or lies inside one");
     RT_DYN_LDS(uint4, lds16);                // 16-byte aligned beside the static variable
     uint16_t *const lds = reinterpret_cast<uint16_t *>(lds16);
-    __shared__ int odd;                      // some value that not every row sees is not finite
     const PagedView &p = a.p;
     const int all_waves = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), split = all_waves / W, wave = all_waves % W;
     const int tid = (int)threadIdx.x - 64 * W * split, lane = tid & 63, j = lane & 31, hh = lane >> 5;
@@ -536,7 +552,6 @@ __global__ __launch_bounds__(64 * W * S, 2) void paged_prefill_kernel(PrefillArg
     const float *qrow = a.q + (size_t)(t0 + tok) * a.q_ld + (size_t)(kvh * a.group + head_in_group) * HD;
     float *orow = a.out + (size_t)(t0 + tok) * a.out_ld + (size_t)(kvh * a.group + head_in_group) * HD;
     const bool has_row = 32 * wave + j < n_rows;
-    if (threadIdx.x == 0) odd = 0;
 
     // ---- the query fragments: lane (j, hh) holds elements 16 kk + 8 hh .. + 7 of its row
     half8v qhi[KK], qlo[KK];
@@ -609,21 +624,15 @@ __global__ __launch_bounds__(64 * W * S, 2) void paged_prefill_kernel(PrefillArg
             vreg[i] = *reinterpret_cast<const u32x4 *>(p.v + at);
         }
     };
-    auto put = [&](int t, int buf, int ok) {             // the requested tile t goes to LDS; values that no row sees as zeros
-        const bool whole = (t + 1) * KT <= least && ok == (1 << (KT / 16)) - 1;
-        if (!whole) {
-            uint32_t found = 0;
+    auto put = [&](int t, int buf, int ok) {             // the requested tile t goes to LDS; values that no row sees (stale, perhaps NaN) as zeros
+        if ((t + 1) * KT > least || ok != (1 << (KT / 16)) - 1) {
 #pragma unroll
             for (int i = 0; i < NL; i++) {
                 const int r = r0 + i * ROWS_AT_ONCE;
                 const bool is = t * KT + r < most && ((ok >> (r >> 4)) & 1);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    vreg[i][e] = is ? vreg[i][e] : 0u;
-                    found |= (uint32_t)((vreg[i][e] & 0x7C00u) == 0x7C00u) | (uint32_t)((vreg[i][e] & 0x7C000000u) == 0x7C000000u);
-                }
+                for (int e = 0; e < 4; e++) vreg[i][e] = is ? vreg[i][e] : 0u;
             }
-            if (found) odd = 1;
         }
 #pragma unroll
         for (int i = 0; i < NL; i++) {
@@ -645,7 +654,6 @@ __global__ __launch_bounds__(64 * W * S, 2) void paged_prefill_kernel(PrefillArg
     if (tiles > 0) {
         request(min(split, tiles - 1));
         ok_now = good;
-        __syncthreads();                                  // odd is cleared before anyone sets it
         put(min(split, tiles - 1), 0, ok_now);
         request(min(S + split, tiles - 1));
         ok_next = good;
@@ -730,15 +738,6 @@ __global__ __launch_bounds__(64 * W * S, 2) void paged_prefill_kernel(PrefillArg
         }
         __syncthreads();
     }
-    if (odd) {
-        for (int row = all_waves; row < n_rows; row += W * S) {
-            int t, h;
-            const int n = place(row, t, h);
-            attend_row<HD>(p, a.q + (size_t)(t0 + t) * a.q_ld + (size_t)(kvh * a.group + h) * HD, a.out + (size_t)(t0 + t) * a.out_ld + (size_t)(kvh * a.group + h) * HD, seq,
-                           kvh, n);
-        }
-        return;
-    }
     l_run += __shfl_xor(l_run, 32);
     if (S > 1) {                                          // the tiles are done with: their memory takes what the groups leave, [value][thread]
         float *left = reinterpret_cast<float *>(lds);
@@ -766,15 +765,30 @@ __global__ __launch_bounds__(64 * W * S, 2) void paged_prefill_kernel(PrefillArg
                 for (int r = 0; r < 16; r++) acc[db][r] = acc[db][r] * keep + its[(16 * db + r) * NT] * add;
         }
     }
-    const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
-    if (!has_row) return;
-    // register r of block db is dim 32 db + 8 (r / 4) + 4 hh + r % 4
+    // rows to be done by themselves: some dim is NaN though the weights are not
+    float sums[4] = { 0.f, 0.f, 0.f, 0.f };
 #pragma unroll
     for (int db = 0; db < DB; db++)
 #pragma unroll
-        for (int g = 0; g < 4; g++)
-            *reinterpret_cast<float4 *>(orow + 32 * db + 8 * g + 4 * hh) =
-                make_float4(acc[db][4 * g] * inv, acc[db][4 * g + 1] * inv, acc[db][4 * g + 2] * inv, acc[db][4 * g + 3] * inv);
+        for (int r = 0; r < 16; r++) sums[r & 3] += acc[db][r];
+    const float sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+    const unsigned long long nan = __ballot(has_row && sum != sum && l_run == l_run);
+    uint32_t again = (uint32_t)nan | (uint32_t)(nan >> 32);
+    const float inv = l_run == 0.f ? 0.f : 1.0f / l_run;
+    // register r of block db is dim 32 db + 8 (r / 4) + 4 hh + r % 4
+    if (has_row && !((again >> j) & 1)) {
+#pragma unroll
+        for (int db = 0; db < DB; db++)
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+                *reinterpret_cast<float4 *>(orow + 32 * db + 8 * g + 4 * hh) =
+                    make_float4(acc[db][4 * g] * inv, acc[db][4 * g + 1] * inv, acc[db][4 * g + 2] * inv, acc[db][4 * g + 3] * inv);
+    }
+    for (; again; again &= again - 1) {
+        int t, h;
+        const int n = place(32 * wave + __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)again) - 1), t, h);
+        attend_row<HD>(p, a.q + (size_t)(t0 + t) * a.q_ld + (size_t)(kvh * a.group + h) * HD, a.out + (size_t)(t0 + t) * a.out_ld + (size_t)(kvh * a.group + h) * HD, seq, kvh, n);
+    }
 }
 
 }  // namespace

@@ -138,3 +138,46 @@ def test_prefill_attention_with_a_bad_first_key_and_a_later_bad_value(ex, bad):
     b.v[b.table[1, 1], 0, 4, 1] = np.nan
     got = prefill(ex, b, queries(rng, "f32", 60, 2 * 64), 2)
     assert np.isnan(got[:30]).any()
+
+
+# ---------------------------------------------------------------------------------------------------------------- values
+
+
+def bad_values(b, s, where):
+    for p, e, x in where:
+        pg, sl = place(b, s, p)
+        b.v[pg, :, sl, e] = x
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("n_kv,n_heads,lens,new", [(2, 4, [200, 90], [40, 90]), (1, 1, [130], [130]), (1, 6, [333], [33])])
+def test_prefill_attention_with_infinite_values_that_are_seen(ex, hd, n_kv, n_heads, lens, new):
+    """A value of infinity that a row sees comes out as that infinity in its dim, both signs or a NaN as NaN, the other dims as ever:
+    far before the rows, among them, and for the row whose only weight it is."""
+    print("prefill, infinite values", hd, n_kv, n_heads, lens, new, flush=True)
+    rng = np.random.default_rng(hd + n_heads)
+    b = ref.Batch(rng, lens, 16, n_kv, hd, new)
+    n = lens[0]
+    bad_values(b, 0, [(0, 1, np.inf), (5, 2, -np.inf), (9, 3, np.nan), (n - 9, 4, np.inf), (n - 20, 4, -np.inf), (n - 7, 60, -np.inf), (n - 1, 7, np.nan)])
+    got = prefill(ex, b, queries(rng, "f32", sum(new), n_heads * hd), n_heads)
+    last = got[new[0] - 1].reshape(n_heads, hd)
+    assert (last[:, 1] == np.inf).all() and (last[:, [2, 60]] == -np.inf).all() and np.isnan(last[:, [3, 4, 7]]).all() and np.isfinite(last[:, 8:60]).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_decode_attention_with_infinite_values(ex, hd):
+    rng = np.random.default_rng(hd)
+    b = ref.Batch(rng, [200, 1, 2000], 16, 2, hd)
+    for s, n in ((0, 200), (1, 1), (2, 2000)):
+        bad_values(b, s, [(0, 1, np.inf), (n // 2, 2, -np.inf), (n - 1, 3, np.nan), (0, 4, np.inf), (n - 1, 4, -np.inf if n > 1 else np.inf)])
+    decode(ex, b, queries(rng, "f32", 3, 4 * hd), 4)
+
+
+def test_prefill_attention_with_infinite_values_and_pages_outside_the_pool(ex):
+    rng = np.random.default_rng(6)
+    b = ref.Batch(rng, [120], 16, 1, 64, [70])
+    b.k[b.table[0, 4]] = b.v[b.table[0, 4]] = np.nan
+    bad_values(b, 0, [(3, 1, np.inf), (70, 2, np.nan), (110, 3, np.inf)])
+    b.table[0, 4] = b.n_pages
+    b.table[0, 2] = -1
+    prefill(ex, b, queries(rng, "f32", 70, 2 * 64), 2)
