@@ -685,10 +685,10 @@ __global__ __launch_bounds__(64 * W * S, 2) void paged_prefill_kernel(PrefillArg
 #pragma unroll
             for (int r = 1; r < 16; r++) mt = fmaxf(mt, s[r]);
             mt = fmaxf(mt, __shfl_xor(mt, 32));
-            mt = fmaxf(m_run, mt * sscale);
+            mt = fmaxf(m_run, mt);                               // running maximum of the products, before the scaling
             const float m_ref = mt == -INFINITY ? 0.f : mt;      // nothing seen yet
             if (__ballot(mt > m_run)) {
-                const float alpha = __builtin_amdgcn_exp2f(m_run - m_ref);
+                const float alpha = __builtin_amdgcn_exp2f((m_run - m_ref) * sscale);
                 l_run *= alpha;
 #pragma unroll
                 for (int db = 0; db < DB; db++)
@@ -699,7 +699,14 @@ __global__ __launch_bounds__(64 * W * S, 2) void paged_prefill_kernel(PrefillArg
             // probabilities times 2^14, so that the lower halves stay normal numbers; both halves are cut, not rounded, which leaves
             // 2^-21 of a probability
             half8v phi[2], plo[2];
-            const float shift = 14.0f - m_ref;
+            float shift = fmaf(-m_ref, sscale, 14.0f);
+            // shift is rounded, to 2^-18 below 128.  Beyond that tiles with another maximum would weigh noticeably differently, and from 2^24 on
+            // the largest weight would be more than an fp16 holds, or nothing: there the differences, at most 0, are taken first.
+            if (__ballot(!(fabsf(shift) < 128.0f))) {
+#pragma unroll
+                for (int r = 0; r < 16; r++) s[r] -= m_ref;
+                shift = 14.0f;
+            }
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
                 const float w0 = __builtin_amdgcn_exp2f(fmaf(s[r], sscale, shift)), w1 = __builtin_amdgcn_exp2f(fmaf(s[r + 1], sscale, shift));
@@ -756,7 +763,7 @@ __global__ __launch_bounds__(64 * W * S, 2) void paged_prefill_kernel(PrefillArg
         for (int o = 0; o < S - 1; o++) {
             const float *its = left + (size_t)o * NV * NT + tid;
             const float m_its = its[16 * DB * NT], m = fmaxf(m_run, m_its), m_ref = m == -INFINITY ? 0.f : m;
-            const float keep = __builtin_amdgcn_exp2f(m_run - m_ref), add = __builtin_amdgcn_exp2f(m_its - m_ref);
+            const float keep = __builtin_amdgcn_exp2f((m_run - m_ref) * sscale), add = __builtin_amdgcn_exp2f((m_its - m_ref) * sscale);
             m_run = m;
             l_run = l_run * keep + its[(16 * DB + 1) * NT] * add;
 #pragma unroll
