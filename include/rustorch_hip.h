@@ -18,7 +18,8 @@
  *     (policy of src/gpu/matrix_ops.rs:408-425).
  *   - `const` pointer arguments are borrowed until the call returns.
  *   - names ending in _dev take device pointers obtained from rt_hip_malloc and
- *     only enqueue work on the context's stream; the other entry points take
+ *     only enqueue work on the context's stream (one of its own, or the
+ *     caller's: rt_hip_create_on_stream); the other entry points take
  *     host pointers and block until the result is in host memory (the contract
  *     of CudaKernelExecutor::matmul_f32, src/gpu/cuda_kernels.rs:231-283).
  *   - a context may be moved between threads; calls on one context are
@@ -93,6 +94,13 @@ RT_HIP_API int rt_hip_device_info(int device, rt_hip_devinfo *out);
 /* ---- executor object: CudaKernelExecutor::new(device_id) and its Drop
  *      (src/gpu/cuda_kernels.rs:211-227, src/gpu/cuda_enhanced.rs:30-60). */
 RT_HIP_API int rt_hip_create(int device, rt_hip_ctx **out);
+/* The same on a stream of the caller's (a hipStream_t of that device; NULL: the device's default stream): what a call enqueues runs in
+ * order with the rest of the caller's work on that stream, so memory that the work before fills, or the work behind reads or reuses,
+ * needs no host wait.  The stream has to outlive the context, which does not destroy it.  While the stream is being captured, calls
+ * that need the context's workspace (it may move in a later call) and rt_hip_memset_dev are refused with RT_HIP_ERR_INVALID_ARG;
+ * calls that wait or copy to or from the host fail as they do in any capture.  The default stream itself cannot be captured: a model on
+ * it has no mode 2 (rt_hip_llama_set_mode). */
+RT_HIP_API int rt_hip_create_on_stream(int device, void *stream, rt_hip_ctx **out);
 RT_HIP_API int rt_hip_destroy(rt_hip_ctx *ctx);
 /* GpuDevice::synchronize (src/gpu/device.rs:9-48). */
 RT_HIP_API int rt_hip_synchronize(rt_hip_ctx *ctx);

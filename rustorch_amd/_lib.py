@@ -32,6 +32,7 @@ SIGNATURES = {
     "rt_hip_device_count": (C.c_int, []),
     "rt_hip_device_info": (C.c_int, [C.c_int, C.POINTER(DevInfo)]),
     "rt_hip_create": (C.c_int, [C.c_int, c_void_pp]),
+    "rt_hip_create_on_stream": (C.c_int, [C.c_int, C.c_void_p, c_void_pp]),
     "rt_hip_destroy": (C.c_int, [C.c_void_p]),
     "rt_hip_synchronize": (C.c_int, [C.c_void_p]),
     "rt_hip_last_error": (C.c_char_p, [C.c_void_p]),

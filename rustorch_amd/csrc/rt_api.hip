@@ -64,8 +64,20 @@ bool set_path_option(int option, int value) {
     return true;
 }
 
+// A context on a stream of its own captures only itself (the model's graph of a decode step); the caller's stream may be in a capture of
+// the caller's, whose graph would keep the workspace's address of that moment.
+int refuse_capture(rt_hip_ctx *ctx, const char *what) {
+    if (ctx->owns_stream || !ctx->stream) return RT_HIP_OK;      // the default stream cannot be captured
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    RT_TRY_HIP(ctx, hipStreamIsCapturing(ctx->stream, &st));
+    RT_REQUIRE(ctx, st == hipStreamCaptureStatusNone, RT_HIP_ERR_INVALID_ARG, "%s cannot be part of a capture of the caller's stream", what);
+    return RT_HIP_OK;
+}
+
 // Grow the context scratch to at least `bytes` (contents are not preserved).
 int ensure_scratch(rt_hip_ctx *ctx, size_t bytes) {
+    int rc = bytes ? refuse_capture(ctx, "a call that needs the context's workspace") : RT_HIP_OK;
+    if (rc) return rc;
     if (ctx->scratch_bytes >= bytes) return RT_HIP_OK;
     if (ctx->scratch) {
         RT_TRY_HIP(ctx, hipStreamSynchronize(ctx->stream));
@@ -125,17 +137,25 @@ int rt_hip_device_info(int device, rt_hip_devinfo *out) {
     return RT_HIP_OK;
 }
 
-int rt_hip_create(int device, rt_hip_ctx **out) {
-    if (!out) return fail(nullptr, RT_HIP_ERR_INVALID_ARG, "rt_hip_create: out is NULL");
+static int create_context(const char *who, int device, bool own_stream, void *stream, rt_hip_ctx **out) {
+    if (!out) return fail(nullptr, RT_HIP_ERR_INVALID_ARG, "%s: out is NULL", who);
     *out = nullptr;
     int n = rt_hip_device_count();
     if (device < 0 || device >= n) return fail(nullptr, RT_HIP_ERR_NO_DEVICE, "hip:%d not available (%d devices)", device, n);
     hipError_t e = hipSetDevice(device);
     if (e != hipSuccess) return hip_fail(nullptr, e, "hipSetDevice");
+    if (stream) {
+        hipDevice_t its = 0;
+        e = hipStreamGetDevice((hipStream_t)stream, &its);
+        if (e != hipSuccess) return hip_fail(nullptr, e, "hipStreamGetDevice");
+        if (its != device) return fail(nullptr, RT_HIP_ERR_INVALID_ARG, "%s: the stream belongs to hip:%d, not hip:%d", who, (int)its, device);
+    }
     rt_hip_ctx *c = new (std::nothrow) rt_hip_ctx();
-    if (!c) return fail(nullptr, RT_HIP_ERR_OOM, "rt_hip_create: host allocation failed");
+    if (!c) return fail(nullptr, RT_HIP_ERR_OOM, "%s: host allocation failed", who);
     c->device = device;
-    e = hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking);
+    c->owns_stream = own_stream;
+    c->stream = (hipStream_t)stream;
+    if (own_stream) e = hipStreamCreateWithFlags(&c->stream, hipStreamNonBlocking);
     if (e != hipSuccess) {
         delete c;
         return hip_fail(nullptr, e, "hipStreamCreate");
@@ -144,13 +164,17 @@ int rt_hip_create(int device, rt_hip_ctx **out) {
     return RT_HIP_OK;
 }
 
+int rt_hip_create(int device, rt_hip_ctx **out) { return create_context("rt_hip_create", device, true, nullptr, out); }
+
+int rt_hip_create_on_stream(int device, void *stream, rt_hip_ctx **out) { return create_context("rt_hip_create_on_stream", device, false, stream, out); }
+
 int rt_hip_destroy(rt_hip_ctx *ctx) {
     if (!ctx) return RT_HIP_OK;
     {
         Guard g(ctx);
         (void)hipStreamSynchronize(ctx->stream);
         if (ctx->scratch) (void)hipFree(ctx->scratch);
-        (void)hipStreamDestroy(ctx->stream);
+        if (ctx->owns_stream) (void)hipStreamDestroy(ctx->stream);
     }
     delete ctx;
     return RT_HIP_OK;
@@ -209,6 +233,8 @@ int rt_hip_memset_dev(rt_hip_ctx *ctx, void *dst_dev, int byte, size_t nbytes) {
     if (!ctx || (nbytes && !dst_dev)) return fail(ctx, RT_HIP_ERR_INVALID_ARG, "rt_hip_memset_dev: NULL argument");
     Guard g(ctx);
     if (!nbytes) return RT_HIP_OK;
+    int rc = rt::refuse_capture(ctx, "rt_hip_memset_dev");
+    if (rc) return rc;
     RT_TRY_HIP(ctx, hipMemsetAsync(dst_dev, byte, nbytes, ctx->stream));
     return RT_HIP_OK;
 }

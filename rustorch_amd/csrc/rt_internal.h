@@ -237,6 +237,7 @@ inline size_t type_block_elems(int t) {
 struct rt_hip_ctx {
     int device = 0;
     hipStream_t stream = nullptr;
+    bool owns_stream = true;       // false: the caller's (rt_hip_create_on_stream)
     std::mutex mu;
     std::string err;
     // scratch owned by the context for the host-pointer entry points and the xq of *_dev GEMV calls
@@ -260,6 +261,7 @@ namespace rt {
 int fail(rt_hip_ctx *ctx, int code, const char *fmt, ...) __attribute__((format(printf, 3, 4)));
 int hip_fail(rt_hip_ctx *ctx, hipError_t e, const char *what);
 int ensure_scratch(rt_hip_ctx *ctx, size_t bytes);
+int refuse_capture(rt_hip_ctx *ctx, const char *what);      // RT_HIP_OK unless the caller's stream is being captured
 
 // Serialises calls on one context and makes its device current.
 struct Guard {

@@ -53,7 +53,8 @@ class DeviceBuffer:
     @classmethod
     def borrow(cls, ex: "HipKernelExecutor", ptr: int, nbytes: int) -> "DeviceBuffer":
         """A buffer over device memory that someone else allocated and keeps (the memory of rt_hip_qweight_wrap_dev is another
-        such case).  The executor's stream is its own: work of another stream on that memory has to be waited for."""
+        such case).  Work of other streams on that memory has to be waited for, unless the executor was made on the stream of that
+        work (HipKernelExecutor's `stream`) and runs in its order."""
         buf = cls.__new__(cls)
         buf.ex, buf.nbytes, buf.ptr, buf.owns = ex, int(nbytes), C.c_void_p(ptr), False
         return buf
@@ -189,11 +190,16 @@ class Event:
 class HipKernelExecutor:
     """`HipKernelExecutor::new(device_id)`; dropped by `close()` or garbage collection."""
 
-    def __init__(self, device_id: int = 0):
+    def __init__(self, device_id: int = 0, stream: int | None = None):
+        """stream: the handle of a stream that the caller keeps (0 is the default stream; torch.cuda.current_stream().cuda_stream), in
+        whose order the calls then run (rt_hip_create_on_stream); None makes one of the executor's own, which nothing else waits for."""
         self.lib = _lib.load()
         self.ctx = C.c_void_p()
         self.device_id = device_id
-        _lib.check(self.lib.rt_hip_create(device_id, C.byref(self.ctx)), None)
+        if stream is None:
+            _lib.check(self.lib.rt_hip_create(device_id, C.byref(self.ctx)), None)
+        else:
+            _lib.check(self.lib.rt_hip_create_on_stream(device_id, stream, C.byref(self.ctx)), None)
 
     # -- lifetime
     def close(self) -> None:

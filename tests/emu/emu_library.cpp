@@ -64,6 +64,10 @@ bool submit(hipStream_t s, std::function<void()> work) {
     return false;
 }
 }  // namespace emu
+hipError_t hipStreamIsCapturing(hipStream_t s, hipStreamCaptureStatus *st) {
+    *st = g_capturing.count(s) ? hipStreamCaptureStatusActive : hipStreamCaptureStatusNone;
+    return hipSuccess;
+}
 hipError_t hipStreamBeginCapture(hipStream_t s, int) {
     if (g_capturing.count(s)) return hipErrorInvalidValue;
     g_capturing[s] = new emu_graph();

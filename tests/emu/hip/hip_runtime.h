@@ -136,6 +136,10 @@ template <class F> inline hipError_t hipFuncSetAttribute(F, int, int) { return h
 template <class T> inline hipError_t hipGetSymbolAddress(void **p, T &symbol) { *p = (void *)&symbol; return hipSuccess; }
 // captured graphs: the list of work recorded between begin and end; a launch of the graph runs the list again
 hipError_t hipStreamBeginCapture(hipStream_t s, int mode);
+enum hipStreamCaptureStatus { hipStreamCaptureStatusNone = 0, hipStreamCaptureStatusActive = 1 };
+typedef int hipDevice_t;
+hipError_t hipStreamIsCapturing(hipStream_t s, hipStreamCaptureStatus *st);
+inline hipError_t hipStreamGetDevice(hipStream_t, hipDevice_t *d) { *d = 0; return hipSuccess; }
 hipError_t hipStreamEndCapture(hipStream_t s, hipGraph_t *g);
 hipError_t hipGraphInstantiate(hipGraphExec_t *e, hipGraph_t g, void *, void *, size_t);
 hipError_t hipGraphLaunch(hipGraphExec_t e, hipStream_t s);

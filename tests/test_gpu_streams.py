@@ -1,0 +1,137 @@
+"""An executor on a stream of the caller's: its calls run in the order of torch's work on that stream, with no host wait between, and a
+capture of that stream either holds them or refuses them."""
+import numpy as np
+import pytest
+
+import paged_ref as ref
+
+pytestmark = pytest.mark.gpu
+
+torch = pytest.importorskip("torch")
+if not torch.cuda.is_available():
+    pytest.skip("needs torch on the device", allow_module_level=True)
+
+from rustorch_amd.errors import InvalidParameters  # noqa: E402
+from rustorch_amd.executor import HipKernelExecutor  # noqa: E402
+
+BUSY = 20_000_000          # device clocks that a stream is kept busy for before the inputs are written: some milliseconds
+
+
+def borrowed(ex, t):
+    return ex.borrow(t.data_ptr(), t.numel() * t.element_size())
+
+
+@pytest.mark.parametrize("which", ["default", "side"])
+def test_calls_run_in_the_order_of_the_callers_stream(which):
+    """Logits that a busy stream writes late are the ones that are sampled, and what torch reads behind the call is its answer; the
+    inputs change again right behind it."""
+    print("order of the stream", which, flush=True)
+    stream = torch.cuda.default_stream() if which == "default" else torch.cuda.Stream()
+    rows, vocab = 4, 50000
+    g = torch.Generator().manual_seed(1)
+    with torch.cuda.stream(stream), HipKernelExecutor(0, stream=stream.cuda_stream) as ex:
+        want = [torch.randint(0, vocab, (rows,), generator=g) for _ in range(5)]
+        late = [torch.nn.functional.one_hot(w, vocab).float().cuda() for w in want]
+        x, u = torch.zeros(rows, vocab, device="cuda"), torch.full((rows,), 0.5, dtype=torch.float64, device="cuda")
+        token, temp = torch.full((rows,), -7, dtype=torch.int32, device="cuda"), torch.zeros(rows, device="cuda")
+        bx, bu, bt, btemp = (borrowed(ex, t) for t in (x, u, token, temp))
+        ex.sample_dev(bx, rows, vocab, bu, bt, temperature=btemp)          # the workspace is there
+        got = []
+        torch.cuda.synchronize()
+        for t in late:
+            torch.cuda._sleep(BUSY)
+            x.copy_(t)
+            ex.sample_dev(bx, rows, vocab, bu, bt, temperature=btemp)
+            got.append(token.clone())
+            x.zero_()
+            token.fill_(-7)
+        stream.synchronize()
+        assert [t.tolist() for t in got] == [w.tolist() for w in want]
+
+
+def test_several_executors_on_one_stream_and_their_ends():
+    """Executors come and go on a stream that stays the caller's."""
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        a = torch.arange(8, dtype=torch.float32, device="cuda")
+        for i in range(3):
+            with HipKernelExecutor(0, stream=stream.cuda_stream) as ex, HipKernelExecutor(0, stream=stream.cuda_stream) as other:
+                for e in (ex, other):
+                    e.add_dev(borrowed(e, a), borrowed(e, a), 8)
+            assert a.tolist() == [v * 4.0 ** (i + 1) for v in range(8)]
+
+
+def paged_case(rng, n_seq_len, new, n_kv, n_heads, hd):
+    b = ref.Batch(rng, n_seq_len, 16, n_kv, hd, new)
+    t = dict(table=b.table, kv_len=b.kv_len, cu=b.cu, k=b.k, v=b.v, q=rng.standard_normal((sum(new), n_heads * hd)).astype(np.float32))
+    return b, {k: torch.from_numpy(np.ascontiguousarray(x)).cuda() for k, x in t.items()}
+
+
+def test_a_capture_of_the_callers_stream_holds_calls_without_a_workspace():
+    """Append and prefill attention captured once, replayed on inputs that change between the replays, with work outside the graph
+    between them: every replay equals the eager calls."""
+    rng = np.random.default_rng(7)
+    n_kv, n_heads, hd = 2, 4, 64
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream), HipKernelExecutor(0, stream=stream.cuda_stream) as ex:
+        b, t = paged_case(rng, [40, 5], [9, 5], n_kv, n_heads, hd)
+        k, v = (torch.randn(14, n_kv * hd, device="cuda") for _ in range(2))
+        qr, out = torch.zeros_like(t["q"]), torch.zeros_like(t["q"])
+        pool = ex.wrap_paged_kv(borrowed(ex, t["k"]), borrowed(ex, t["v"]), b.n_pages, 16, n_kv, hd)
+        seqs = ex.paged_seqs(borrowed(ex, t["table"]), borrowed(ex, t["kv_len"]), 2, b.max_blocks, borrowed(ex, t["cu"]))
+        bk, bv, bq, bqr, bout = (borrowed(ex, x) for x in (k, v, t["q"], qr, out))
+
+        def step():
+            ex.paged_append_dev(pool, seqs, bk, bv, 14, q=bq, q_out=bqr, n_heads=n_heads)
+            ex.paged_attn_prefill_dev(pool, seqs, bqr, 14, n_heads, bout)
+
+        step()
+        stream.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            step()
+        for i in range(4):
+            for x in (k, v, t["q"]):
+                x.normal_()
+            out.zero_()
+            graph.replay()
+            replayed, pages = out.clone(), t["k"].clone()
+            out.zero_()
+            t["k"].view(torch.int16)[:, :, 5:7] ^= 0                       # work of the caller's own
+            step()
+            stream.synchronize()
+            assert torch.equal(replayed, out) and torch.equal(pages, t["k"]) and bool((out != 0).any())
+
+
+def test_a_capture_of_the_callers_stream_refuses_what_it_cannot_keep():
+    """A split decode step and a large sampling need the workspace, which may move later; a memset is no part of a graph here.  The
+    capture goes on without them, and the calls work before and behind it."""
+    rng = np.random.default_rng(8)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream), HipKernelExecutor(0, stream=stream.cuda_stream) as ex:
+        b, t = paged_case(rng, [1500, 30], [1, 1], 1, 2, 64)
+        pool = ex.wrap_paged_kv(borrowed(ex, t["k"]), borrowed(ex, t["v"]), b.n_pages, 16, 1, 64)
+        seqs = ex.paged_seqs(borrowed(ex, t["table"]), borrowed(ex, t["kv_len"]), 2, b.max_blocks, None, 1500)
+        out = torch.zeros_like(t["q"])
+        x, u, token = torch.zeros(2, 40000, device="cuda"), torch.zeros(2, dtype=torch.float64, device="cuda"), torch.zeros(2, dtype=torch.int32, device="cuda")
+        bq, bout, bx, bu, bt = (borrowed(ex, y) for y in (t["q"], out, x, u, token))
+        a = torch.ones(4, device="cuda")
+        ba = borrowed(ex, a)
+        ex.paged_attn_decode_dev(pool, seqs, bq, 2, bout)
+        first = out.clone()
+        stream.synchronize()
+        graph, refused = torch.cuda.CUDAGraph(), 0
+        with torch.cuda.graph(graph, stream=stream):
+            for call in (lambda: ex.paged_attn_decode_dev(pool, seqs, bq, 2, bout), lambda: ex.sample_dev(bx, 2, 40000, bu, bt), lambda: bout.zero()):
+                try:
+                    call()
+                except InvalidParameters as e:
+                    refused += "capture" in str(e)
+            ex.add_dev(ba, ba, 4)
+        assert refused == 3
+        for i in range(3):
+            graph.replay()
+            out.zero_()
+            ex.paged_attn_decode_dev(pool, seqs, bq, 2, bout)
+            stream.synchronize()
+            assert torch.equal(out, first) and a.tolist() == [2.0 ** (i + 1)] * 4
