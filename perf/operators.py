@@ -18,16 +18,17 @@ import torch
 own = False
 
 DEV = "cuda"
-_ex = None
+_ex = {}
 
 
 def _executor():
-    """One executor for the process, as a server has."""
-    global _ex
-    if _ex is None:
+    """One executor for the process, as a server has, on the stream that makes the inputs and reads the outputs: its calls run in
+    the order of torch's work."""
+    stream = torch.cuda.current_stream().cuda_stream
+    if stream not in _ex:
         from rustorch_amd.executor import HipKernelExecutor
-        _ex = HipKernelExecutor(0)
-    return _ex
+        _ex[stream] = HipKernelExecutor(0, stream=stream)
+    return _ex[stream]
 
 
 # ------------------------------------------------------------------------------------------------------------ the cases
@@ -177,7 +178,8 @@ def prepare(case, seed):
 
 def _wrap(st):
     """The handles that a user's program keeps: device buffers over the tensors, the page pool, the batch's description."""
-    ex, c = _executor(), st["case"]
+    st["ex"], c = _executor(), st["case"]
+    ex = st["ex"]
     st["buf"] = b = {k: ex.borrow(t.data_ptr(), t.numel() * t.element_size()) for k, t in st.items() if isinstance(t, torch.Tensor)}
     if c["op"] != "sample":
         st["pool"] = ex.wrap_paged_kv(b["k_pages"], b["v_pages"], st["k_pages"].shape[0], c["page"], c["kv"], c["hd"])
@@ -300,7 +302,7 @@ def run(state):
     c = state["case"]
     if not own:
         return _PLAIN[c["op"]](state)
-    ex, b = _executor(), state["buf"]
+    ex, b = state["ex"], state["buf"]
     if c["op"] == "append":
         ex.paged_append_dev(state["pool"], state["seqs"], b["k"], b["v"], state["q"].shape[0], q=b["q"], q_out=b["out"], n_heads=c["heads"], rope=c["rope"], theta=c["theta"])
         return {"q": state["out"], "k_pages": state["k_pages"], "v_pages": state["v_pages"]}
