@@ -45,18 +45,19 @@ class DeviceBuffer:
     def __init__(self, ex: "HipKernelExecutor", nbytes: int):
         self.ex = ex
         self.nbytes = int(nbytes)
-        self.owns = True
+        self.owns, self.keep = True, None
         p = C.c_void_p()
         _lib.check(ex.lib.rt_hip_malloc(ex.ctx, self.nbytes, C.byref(p)), ex.ctx)
         self.ptr = p
 
     @classmethod
-    def borrow(cls, ex: "HipKernelExecutor", ptr: int, nbytes: int) -> "DeviceBuffer":
+    def borrow(cls, ex: "HipKernelExecutor", ptr: int, nbytes: int, keep=None) -> "DeviceBuffer":
         """A buffer over device memory that someone else allocated and keeps (the memory of rt_hip_qweight_wrap_dev is another
         such case).  Work of other streams on that memory has to be waited for, unless the executor was made on the stream of that
-        work (HipKernelExecutor's `stream`) and runs in its order."""
+        work (HipKernelExecutor's `stream`) and runs in its order.  keep: the memory's owner, where it would otherwise go with its last
+        name (a larger buffer that this is a part of)."""
         buf = cls.__new__(cls)
-        buf.ex, buf.nbytes, buf.ptr, buf.owns = ex, int(nbytes), C.c_void_p(ptr), False
+        buf.ex, buf.nbytes, buf.ptr, buf.owns, buf.keep = ex, int(nbytes), C.c_void_p(ptr), False, keep
         return buf
 
     @classmethod
@@ -86,7 +87,7 @@ class DeviceBuffer:
         if self.ptr:
             if self.owns:
                 self.ex.lib.rt_hip_free(self.ex.ctx, self.ptr)
-            self.ptr = C.c_void_p()
+            self.ptr, self.keep = C.c_void_p(), None
 
     def __del__(self):
         try:
@@ -126,10 +127,10 @@ class PagedKV:
         self.nbytes = 2 * n_pages * page_size * n_kv_heads * head_dim       # of the keys, and of the values
 
     def pages(self) -> tuple[DeviceBuffer, DeviceBuffer]:
-        """The key pages and the value pages as buffers that this pool keeps."""
+        """The key pages and the value pages as buffers over the pool's memory, which live as long as they do (or until free())."""
         k, v = C.c_void_p(), C.c_void_p()
         _lib.check(self.ex.lib.rt_hip_paged_kv_pages(self.ex.ctx, self.handle, C.byref(k), C.byref(v)), self.ex.ctx)
-        return DeviceBuffer.borrow(self.ex, k.value, self.nbytes), DeviceBuffer.borrow(self.ex, v.value, self.nbytes)
+        return DeviceBuffer.borrow(self.ex, k.value, self.nbytes, self), DeviceBuffer.borrow(self.ex, v.value, self.nbytes, self)
 
     def free(self) -> None:
         if self.handle:
@@ -244,9 +245,9 @@ class HipKernelExecutor:
     def event(self) -> Event:
         return Event(self)
 
-    def borrow(self, ptr: int, nbytes: int) -> DeviceBuffer:
+    def borrow(self, ptr: int, nbytes: int, keep=None) -> DeviceBuffer:
         """A buffer over device memory allocated elsewhere; see DeviceBuffer.borrow."""
-        return DeviceBuffer.borrow(self, ptr, nbytes)
+        return DeviceBuffer.borrow(self, ptr, nbytes, keep)
 
     def buffer(self, nbytes: int) -> DeviceBuffer:
         return DeviceBuffer(self, nbytes)

@@ -12,7 +12,7 @@ sys.path.insert(0, str(ROOT / "tests" / "emu"))
 import build_emulated  # noqa: E402
 
 needs_rocm = pytest.mark.skipif(not (Path(build_emulated.CLANG).exists() and shutil.which("gcc")), reason="needs ROCm's clang++ and gcc")
-SELECTION = ["tests/test_gpu_paged_nonfinite.py", "tests/test_gpu_paged_scores.py"]
+SELECTION = ["tests/test_gpu_paged_nonfinite.py", "tests/test_gpu_paged_scores.py", "tests/test_gpu_paged_handles.py"]
 
 
 @needs_rocm
