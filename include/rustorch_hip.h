@@ -265,7 +265,7 @@ RT_HIP_API int rt_hip_argmax_dev(rt_hip_ctx *ctx, const float *v, size_t n, int 
  *      Sequences may share pages that are only read.  A call takes up to 65535 sequences of up to 2^30 positions, append up to 2^22
  *      tokens, decode up to 2^22 rows times query heads, prefill up to 65535 * 64 rows of tokens times query heads per key / value
  *      head.  Rows of q, k, v and the outputs are *_ld floats apart (a multiple of 4, at
- *      least the row's length), their bases 16-byte aligned; query head h reads key / value head h / (n_heads / n_kv_heads). */
+ *      least the row's length, at most 2^38), their bases 16-byte aligned; query head h reads key / value head h / (n_heads / n_kv_heads). */
 RT_HIP_API int rt_hip_paged_kv_create(rt_hip_ctx *ctx, size_t n_pages, int page_size, int n_kv_heads, int head_dim, rt_hip_paged_kv **out);
 RT_HIP_API int rt_hip_paged_kv_wrap_dev(rt_hip_ctx *ctx, uint16_t *k_pages, uint16_t *v_pages, size_t n_pages, int page_size, int n_kv_heads,
                                         int head_dim, rt_hip_paged_kv **out);
@@ -299,7 +299,7 @@ RT_HIP_API int rt_hip_paged_attn_prefill_dev(rt_hip_ctx *ctx, const rt_hip_paged
                                              size_t out_ld);
 
 /* ---- sampling on the device: SamplingConfig's temperature, top-k and top-p (example-cli/src/model/sampling.rs:8-80,118-274)
- *      and min-p, one token per row of logits (rows ld floats apart) from given random numbers u in [0, 1).  The settings are
+ *      and min-p, one token per row of logits (rows ld floats apart, at most 2^38) from given random numbers u in [0, 1).  The settings are
  *      device arrays of one value per row; NULL, or a value that means nothing, switches a filter off: temperature <= 0 or
  *      top_k 1 is the greedy pick (ties: lowest index; NULL temperature is 1), top_k <= 0, top_p outside (0, 1), min_p <= 0
  *      are off.  The kept tokens: the top_k largest (equal logits: lower index first), of these the shortest prefix whose

@@ -18,6 +18,8 @@ namespace rt {
 constexpr double kHbmPeakBytesPerSec = 8.0e12;
 constexpr double kMfmaF16PeakFlops = 2.5e15;
 constexpr int kWave = 64;
+// floats between two rows of a strided argument: beyond this it is a negative number that became a size_t
+constexpr size_t kRowsApartMost = (size_t)1 << 38;
 
 // ---- quantized activation vector ("xq"): what the GEMV kernels consume.
 // A vector of K floats (K % 32 == 0) is stored per 32-element block as

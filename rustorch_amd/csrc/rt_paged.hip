@@ -134,7 +134,8 @@ int batch_check(rt_hip_ctx *ctx, const char *who, const rt_hip_paged_kv *kv, con
 
 int rows_check(rt_hip_ctx *ctx, const char *who, const char *name, const void *p, size_t ld, size_t least) {
     RT_REQUIRE(ctx, ((uintptr_t)p & 15) == 0, RT_HIP_ERR_INVALID_ARG, "%s: %s must be 16-byte aligned", who, name);
-    RT_REQUIRE(ctx, ld >= least && ld % 4 == 0, RT_HIP_ERR_SHAPE, "%s: rows of %s are %zu floats apart (at least %zu, a multiple of 4)", who, name, ld, least);
+    RT_REQUIRE(ctx, ld >= least && ld <= rt::kRowsApartMost && ld % 4 == 0, RT_HIP_ERR_SHAPE, "%s: rows of %s are %zu floats apart (at least %zu, a multiple of 4)", who, name, ld,
+               least);
     return RT_HIP_OK;
 }
 

@@ -892,7 +892,7 @@ int rt_hip_sample_dev(rt_hip_ctx *ctx, const float *logits, size_t ld, int n_row
     RT_REQUIRE(ctx, logits && u && out_token, RT_HIP_ERR_INVALID_ARG, "sample: NULL argument");
     RT_REQUIRE(ctx, n_rows >= 0 && n_rows <= 65535, RT_HIP_ERR_SHAPE, "sample: n_rows=%d outside 0..65535", n_rows);
     RT_REQUIRE(ctx, vocab >= 1 && vocab <= (1 << 20), RT_HIP_ERR_SHAPE, "sample: vocab=%d outside 1..2^20", vocab);
-    RT_REQUIRE(ctx, ld >= (size_t)vocab, RT_HIP_ERR_SHAPE, "sample: rows are %zu floats apart, vocab=%d", ld, vocab);
+    RT_REQUIRE(ctx, ld >= (size_t)vocab && ld <= rt::kRowsApartMost, RT_HIP_ERR_SHAPE, "sample: rows are %zu floats apart, vocab=%d", ld, vocab);
     if (n_rows == 0) return RT_HIP_OK;
     Guard g(ctx);
     int bits = 0;

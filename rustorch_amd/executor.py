@@ -160,6 +160,8 @@ class PagedSeqs:
 def _rows(what: str, buf: DeviceBuffer, rows: int, row: int, ld: int | None) -> int:
     """The distance between rows in floats, after checking that the buffer holds `rows` of them."""
     ld = row if ld is None else ld
+    if ld < row:
+        raise ShapeMismatch("%s: rows of %d floats, %d apart" % (what, row, ld))
     if rows and buf.nbytes < 4 * ((rows - 1) * ld + row):
         raise ShapeMismatch("%s: a buffer of %d bytes for %d rows of %d floats, %d apart" % (what, buf.nbytes, rows, row, ld))
     return ld
