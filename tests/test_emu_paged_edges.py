@@ -12,7 +12,7 @@ sys.path.insert(0, str(ROOT / "tests" / "emu"))
 import build_emulated  # noqa: E402
 
 needs_rocm = pytest.mark.skipif(not (Path(build_emulated.CLANG).exists() and shutil.which("gcc")), reason="needs ROCm's clang++ and gcc")
-SELECTION = ["tests/test_gpu_paged_nonfinite.py", "tests/test_gpu_paged_scores.py", "tests/test_gpu_paged_handles.py",
+SELECTION = ["tests/test_gpu_paged_nonfinite.py", "tests/test_gpu_paged_scores.py", "tests/test_gpu_paged_handles.py", "tests/test_gpu_sample_bounds.py",
              "tests/test_gpu_paged_forms.py::test_prefill_attention_of_128_rows_a_workgroup[640-640-16-new0-prior0-1.0]",
              "tests/test_gpu_paged_forms.py::test_decode_attention_over_more_pages_than_lanes[1-2-kv_len0-1-64]",
              "tests/test_gpu_paged_forms.py::test_decode_attention_over_more_pages_than_lanes[1-2-kv_len0-1-128]"]
