@@ -306,7 +306,7 @@ RT_HIP_API int rt_hip_paged_attn_prefill_dev(rt_hip_ctx *ctx, const rt_hip_paged
  *      probability reaches top_p of theirs, of these the ones at least min_p times as likely as the largest; the draw is the
  *      first kept token by index whose running probability exceeds u.  NaN logits count as -inf; a row with nothing above -inf
  *      reports -1.  out_prob (may be NULL): the probability the token was drawn with.  Probabilities are summed exactly,
- *      as integers in units of 2^-F of the largest, F = 62 - ceil(log2(vocab)) and at most 51: a token at least 2^-(F + 1) times as likely
+ *      as integers in units of 2^-F of the largest, F = 62 - ceil(log2(vocab)) and at most 51: a token more than 2^-(F + 1) times as likely
  *      as the largest can be drawn, a less likely one never is (2^-52 up to 2048 tokens, 2^-46 for 131072, 2^-43 for 2^20).  vocab up to
  *      2^20. */
 RT_HIP_API int rt_hip_sample_dev(rt_hip_ctx *ctx, const float *logits, size_t ld, int n_rows, int vocab, const float *temperature, const int *top_k,

@@ -30,7 +30,7 @@ typedef float float4v __attribute__((ext_vector_type(4)));
 // the chunk counts (64 sequences at a time, one load and a few lane exchanges).  A sequence of one chunk is finished at once;
 // the chunks of a longer one are joined by paged_join_kernel.
 // Measured (keys and values of three batches in turn, so that none stay in the last-level cache): 537 MB of one sequence of 131071
-// positions 95.5 us (5.6 TB/s), 837 MB of 48 sequences 163 us (5.1 TB/s), 278 MB of 33 sequences 63 us (4.4 TB/s), join included;
+// positions 95.3 us (5.6 TB/s), 837 MB of 48 sequences 163 us (5.1 TB/s), 278 MB of 33 sequences 64 us (4.4 TB/s), join included;
 // the join alone takes 4 to 5 us.  A copy of 4 GiB moves 4.6 TB/s.
 constexpr int kDecodeWaves = 4, kChunkUnit = 128, kHeadsPerBlock = 16, kChunkMinUnits = 2;
 
@@ -352,8 +352,8 @@ __global__ __launch_bounds__(kJoinThreads) void paged_join_kernel(DecodeArgs a) 
 }
 
 // Chunks beyond one per sequence that a launch may cut (0: none, and no join).
-//   * No position count above 256: every sequence is one chunk.  One chat of 200 positions, 32 heads: 8.5 us; cut in two and
-//     joined, 9.5 us.
+//   * No position count above 256: every sequence is one chunk.  One chat of 200 positions, 32 heads: 8.6 us; cut in two and
+//     joined, 11.0 us.
 //   * Several sequences: about 1536 workgroups, two rounds of the three that a compute unit holds.  33 sequences of 1 to 4097
 //     positions, 8 kv heads: 71 us with 512 workgroups, 66 with 1024, 63 with 1536 and 2048; 48 sequences of 1000 to 16000, 4 kv
 //     heads: 188, 176, 163, 167.
@@ -416,8 +416,8 @@ namespace {
 // at one that it sees, where a half of the probability is zero.  Rows whose outputs are NaN at the end though their weights are not
 // are done again by themselves (attend_row), where a value meets its weight once and only if it is seen: nothing in the loop
 // over the tiles looks for such values.  A weight that f32 cannot hold (below 2^-149 of the largest) is zero there too, and NaN with them.
-// Measured: one prompt of 8191 tokens, 32 heads over 8 kv heads of 128: 1.05 ms = 524 TFLOP/s of the formula, 1048 of fp16 products (a
-// library product of 8192^3 reaches 1139); a prompt of 512, 32 kv heads: 21.8 us.
+// Measured: one prompt of 8191 tokens, 32 heads over 8 kv heads of 128: 1.04 ms = 529 TFLOP/s of the formula, 1059 of fp16 products (a
+// library product of 8192^3 reaches 1139); a prompt of 512, 32 kv heads: 21.9 us.
 constexpr int kPrefillKeys = 32;
 
 struct PrefillArgs {
@@ -501,7 +501,7 @@ __global__ __launch_bounds__(64 * W * S, 2) void paged_prefill_kernel(PrefillArg
     const int kvh = blockIdx.x, tile = (int)blockIdx.y;
 
     // ---- which rows.  Up to 64 sequences: the one with the most positions first, and of each its last rows first, which see the most
-    // (a long one that began last would end alone: six chunks behind prefixes of 0 to 3000 take 114 instead of 138 us).  More: sequence s
+    // (a long one that began last would end alone: six chunks behind prefixes of 0 to 3000 take 107 instead of 132 us).  More: sequence s
     // has the tiles from floor(cu_new[s] * group / TQ) + s on, the last first.
     int seq = 0, nth;
     if (p.n_seq <= 64) {
@@ -815,9 +815,9 @@ hipError_t launch_paged_prefill(hipStream_t s, const PagedView &p, int head_dim,
     // 128 rows a workgroup and two of those per compute unit read the keys least often; with fewer than two and a half such workgroups
     // per compute unit, 64 rows and two groups of waves that share the positions end sooner (32 heads of 128, one prompt; us):
     //   tokens          64   256   512  1024  2048  3000  4096  6000
-    //   128 rows       9.0  19.9  31.9  54.8   108   179   317   630
-    //   64 rows, two   9.4  14.7  21.8  38.1   101   198   347   726
-    // Heads of 64 take half the registers and LDS, and the smaller form throughout (16 heads, 6000 tokens: 205 for 220 us).
+    //   128 rows       9.1  19.5  30.7  51.4   100   172   303   583
+    //   64 rows, two   9.8  15.1  22.4  38.2    96   185   323   666
+    // Heads of 64 take half the registers and LDS, and the smaller form throughout (16 heads, 6000 tokens: 192 us, 194 with 128 rows).
     if (head_dim == 64) return run_prefill<64, 2, 2>(s, a);
     if ((long long)n_tok * a.group / 128 * p.n_kv >= 640) return run_prefill<128, 4, 1>(s, a);
     return run_prefill<128, 2, 2>(s, a);

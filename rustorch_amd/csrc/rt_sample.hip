@@ -10,10 +10,11 @@
 // the draw do not depend on how the row is split over threads, and a token is lost to rounding only below 2^-(F+1) of the
 // largest weight (F = 45 for a vocabulary of 131072).  32-bit sums would move the cuts of a large vocabulary by whole tokens.
 //
-// Four launches.  sample_range_kernel finds each row's largest and smallest logit, sample_histogram_kernel counts
+// Large vocabularies take four launches.  sample_range_kernel finds each row's largest and smallest logit, sample_histogram_kernel counts
 // and weighs the tokens by how far below it they are, sample_collect_kernel finds from the histogram the bins that the cuts fall
 // into, lists the tokens of just those bins and sums the weights of the tokens above them, sample_finish_kernel ranks the listed
-// tokens exactly and draws.  The first three split a row over as many workgroups as fill the device.
+// tokens exactly and draws.  The first three split a row over as many workgroups as fill the device.  Up to 32768 tokens one workgroup
+// does all of it for its row in one launch (sample_row_kernel).
 #include "rt_device.h"
 
 #include <algorithm>
@@ -145,7 +146,7 @@ __device__ __forceinline__ RowBins row_bins(float top, float low, double T, int 
     b.rate = 1.4426950408889634 / T;
     b.topf = top;
     b.half_top = 0.5f * top;      // half of d always fits f32
-    b.scale = R > 0.0 ? fminf(2.0f * (float)(kBins - 1) / (float)(0.5 * R) * 0.5f, 1e37f) : 0.0f;
+    b.scale = R > 0.0 ? fminf((float)(kBins - 1) / (float)(0.5 * R), 1e37f) : 0.0f;
     b.frac_bits = frac_bits;
     return b;
 }
@@ -505,8 +506,9 @@ __global__ __launch_bounds__(kThreads) void sample_collect_kernel(SampleArgs a, 
 }
 
 // The row on its own, without bins: the cuts by bisection over the 32 bits of the logits' order, one pass over the row per bit.
-// For rows with infinite logits and for rows with more equal or nearly equal logits in one bin than the list of
-// finish_row holds.  run: kThreads entries, tie as many.
+// For rows with infinite logits and for rows with more equal or nearly equal logits in the cuts' bins than the list of
+// finish_row holds: right, and slow (one row of 32000 equal logits with top-p 180 us; 128256 that were once bf16, so flat that thousands
+// share a bin, 6 ms where 40 us are usual).  run: kThreads entries, tie as many.
 template <int kThreads>
 __device__ void sample_by_bisection(const SampleArgs &a, int r, const RowAsks &q, float top, unsigned long long *run, int *tie, unsigned long long *red) {
     const int tid = threadIdx.x, V = a.vocab, k = q.k > 0 ? q.k : V;
@@ -902,6 +904,8 @@ int rt_hip_sample_dev(rt_hip_ctx *ctx, const float *logits, size_t ld, int n_row
     //   rows x vocab    1 x 32000   64 x 32000  256 x 32000  64 x 65536  77 x 131071  1 x 131071
     //   one launch      23/42/23    24/44/24    28/47/27     34/73/39    59/135/73    50/127/65
     //   four            26/31/21    40/55/27    55/78/42     39/53/30    50/78/43     30/36/20
+    // The rule looks at the vocabulary alone.  Up to 32768 tokens one launch is the faster from 64 rows on and needs no workspace; it costs a
+    // single row up to 11 us with top-p alone.  Above, four are the faster but for a small top-k, which loses up to 5 us at 64 rows.
     if (vocab <= 32768) {
         rt::sample_row_kernel<<<dim3((unsigned)n_rows), rt::kRowThreads, 0, ctx->stream>>>(a);
         RT_TRY_HIP(ctx, hipGetLastError());
@@ -909,7 +913,7 @@ int rt_hip_sample_dev(rt_hip_ctx *ctx, const float *logits, size_t ld, int n_row
     }
     // A row is split so that about a thousand workgroups look for the ranges (2048 tokens at least in each) and as many as there are
     // compute units count (4096 tokens at least): every one of the latter adds up to 4096 bins to the row's histogram.  77 rows
-    // of 131071: 71 us with 256 workgroups, 73 with 512, 81 with 1024.  Rows go in groups whose histograms stay below 64 MB.
+    // of 131071 with 256, 512 and 1024 workgroups: top-p 0.9 78, 88 and 105 us, top-k 40 and top-p 0.95 50, 56 and 69.  Rows go in groups whose histograms stay below 64 MB.
     const int group = std::min(n_rows, 1024);
     rt::SampleWork w;
     w.splits = std::max(1, std::min(1024 / group, (vocab + 2047) / 2048));
