@@ -97,9 +97,10 @@ RT_HIP_API int rt_hip_create(int device, rt_hip_ctx **out);
 /* The same on a stream of the caller's (a hipStream_t of that device; NULL: the device's default stream): what a call enqueues runs in
  * order with the rest of the caller's work on that stream, so memory that the work before fills, or the work behind reads or reuses,
  * needs no host wait.  The stream has to outlive the context, which does not destroy it.  While the stream is being captured, calls
- * that need the context's workspace (it may move in a later call) and rt_hip_memset_dev are refused with RT_HIP_ERR_INVALID_ARG;
+ * that need the context's workspace (it may move in a later call), a model's steps and prompts, and rt_hip_memset_dev are refused with
+ * RT_HIP_ERR_INVALID_ARG;
  * calls that wait or copy to or from the host fail as they do in any capture.  The default stream itself cannot be captured: a model on
- * it has no mode 2 (rt_hip_llama_set_mode). */
+ * it refuses mode 2 (rt_hip_llama_set_mode). */
 RT_HIP_API int rt_hip_create_on_stream(int device, void *stream, rt_hip_ctx **out);
 RT_HIP_API int rt_hip_destroy(rt_hip_ctx *ctx);
 /* GpuDevice::synchronize (src/gpu/device.rs:9-48). */

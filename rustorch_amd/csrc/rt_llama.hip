@@ -707,6 +707,7 @@ int rt_hip_llama_set_mode(rt_hip_ctx *ctx, rt_hip_llama *m, int mode) {
     // The persistent step kernel took a GPU memory fault on its first run and the cause has not been found:
     // the path stays switched off until it is, and asking for it is an error rather than a silent fallback.
     RT_REQUIRE(ctx, mode != 0, RT_HIP_ERR_UNSUPPORTED_TYPE, "persistent step kernel is switched off in this build (unresolved GPU memory fault)");
+    RT_REQUIRE(ctx, mode != 2 || ctx->stream, RT_HIP_ERR_INVALID_ARG, "mode 2 captures its stream, and the device's default stream cannot be captured");
     Guard g(ctx);
     m->mode = mode;
     if (mode != 2) drop_step_graphs(m);
@@ -721,6 +722,8 @@ int rt_hip_llama_step(rt_hip_ctx *ctx, rt_hip_llama *m, int token, int pos, int 
     int rc = check_complete(ctx, m);
     if (rc) return rc;
     Guard g(ctx);
+    rc = rt::refuse_capture(ctx, "a model step");             // the count of fed tokens moves once, not with every replay
+    if (rc) return rc;
     RT_TRY_HIP(ctx, rt::launch_set_state(ctx->stream, m->state, pos, token, 0));
     rc = enqueue_token(ctx, m, true, false, false);
     if (rc) return rc;
@@ -743,6 +746,8 @@ int rt_hip_llama_prefill(rt_hip_ctx *ctx, rt_hip_llama *m, const int *tokens, in
     int rc = check_complete(ctx, m);
     if (rc) return rc;
     Guard g(ctx);
+    rc = rt::refuse_capture(ctx, "a model step");
+    if (rc) return rc;
     if (n_tok >= kPrefillMinRows && prefill_batchable(m)) {
         // dense-contraction path, kPrefillChunk tokens per pass; the logits of the last token come from the head GEMV
         rc = ensure_prefill_buffers(ctx, m, std::min((size_t)n_tok, kPrefillChunk));
@@ -810,6 +815,8 @@ int rt_hip_llama_decode(rt_hip_ctx *ctx, rt_hip_llama *m, int first_token, int p
     int rc = check_complete(ctx, m);
     if (rc) return rc;
     Guard g(ctx);
+    rc = rt::refuse_capture(ctx, "a model step");
+    if (rc) return rc;
     if (forced) {
         RT_TRY_HIP(ctx, hipMemcpyAsync(m->forced_dev, forced, (size_t)n_steps * sizeof(int), hipMemcpyHostToDevice, ctx->stream));
         RT_TRY_HIP(ctx, hipStreamSynchronize(ctx->stream));
@@ -898,6 +905,8 @@ int rt_hip_llama_batch_step(rt_hip_ctx *ctx, rt_hip_llama_batch *b, const int *t
     int rc = check_complete(ctx, m);
     if (rc) return rc;
     Guard g(ctx);
+    rc = rt::refuse_capture(ctx, "a model step");
+    if (rc) return rc;
     const size_t bytes = (size_t)b->n_seq * sizeof(int);
     // (pageable host memory: the copies have left tok / pos when the calls return)
     RT_TRY_HIP(ctx, hipMemcpyAsync(b->tok, tok, bytes, hipMemcpyHostToDevice, ctx->stream));
@@ -928,6 +937,8 @@ int rt_hip_llama_batch_prefill(rt_hip_ctx *ctx, rt_hip_llama_batch *b, int seq, 
     int rc = check_complete(ctx, m);
     if (rc) return rc;
     Guard g(ctx);
+    rc = rt::refuse_capture(ctx, "a model step");
+    if (rc) return rc;
     rc = ensure_prefill_buffers(ctx, m, std::min((size_t)n_tok, kPrefillChunk));
     if (rc) return rc;
     // the model's own passes, writing and attending this sequence's cache for the length of the call

@@ -135,3 +135,69 @@ def test_a_capture_of_the_callers_stream_refuses_what_it_cannot_keep():
             ex.paged_attn_decode_dev(pool, seqs, bq, 2, bout)
             stream.synchronize()
             assert torch.equal(out, first) and a.tolist() == [2.0 ** (i + 1)] * 4
+
+
+CFG = dict(n_layers=2, hidden=256, n_heads=2, ffn=512, vocab=128, max_pos=24)
+
+
+def walk(ex, mode):
+    """Picks and logits of a small model over a prompt, steps and a decode."""
+    from rustorch_amd import llama
+    m = llama.HipLlama(ex, **CFG)
+    llama.load_synthetic(m, 5)
+    m.set_mode(mode)
+    m.prefill([3, 77, 100, 9, 14], 0)
+    picks = [m.step(t, 5 + i) for i, t in enumerate((1, 2, 3, 4))]
+    out = picks, m.decode(picks[-1], 9, 6).tolist(), m.logits()
+    m.close()
+    return out
+
+
+@pytest.mark.parametrize("which,mode", [("default", 1), ("side", 1), ("side", 2)])
+def test_a_model_on_the_callers_stream(ex, which, mode):
+    """The same picks and logits, bit for bit, as on a stream of the executor's own."""
+    stream = torch.cuda.default_stream() if which == "default" else torch.cuda.Stream()
+    want = walk(ex, 1)
+    with torch.cuda.stream(stream), HipKernelExecutor(0, stream=stream.cuda_stream) as mine:
+        got = walk(mine, mode)
+    assert got[:2] == want[:2] and np.array_equal(got[2], want[2])
+
+
+def test_a_model_refuses_the_graphs_that_cannot_be():
+    """Mode 2 on the default stream, which cannot be captured, and a step inside a capture of the caller's, whose replays would not count
+    the tokens; the model goes on as before."""
+    from rustorch_amd import llama
+    with HipKernelExecutor(0, stream=0) as mine:
+        m = llama.HipLlama(mine, **CFG)
+        with pytest.raises(InvalidParameters, match="default stream"):
+            m.set_mode(2)
+        m.close()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream), HipKernelExecutor(0, stream=stream.cuda_stream) as mine:
+        m = llama.HipLlama(mine, **CFG)
+        llama.load_synthetic(m, 5)
+        b = llama.HipLlamaBatch(m, 3, 24)
+        first = m.step(3, 0)
+        a = torch.ones(4, device="cuda")
+        ba = borrowed(mine, a)
+        graph, refused = torch.cuda.CUDAGraph(), 0
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            for call in (lambda: m.step(7, 1, want_token=False), lambda: m.prefill([1, 2, 3], 1), lambda: m.decode(1, 1, 2), lambda: b.step([1, 2, 3], [0, 0, 0], want_tokens=False),
+                         lambda: b.prefill(0, [1, 2, 3])):
+                try:
+                    call()
+                except InvalidParameters as e:
+                    refused += "capture" in str(e)
+            mine.add_dev(ba, ba, 4)
+        graph.replay()
+        stream.synchronize()
+        assert refused == 5 and a.tolist() == [2.0] * 4
+        m.step(7, 1)
+        got = m.logits()
+        m.reset()
+        assert m.step(3, 0) == first
+        m.step(7, 1)
+        assert np.array_equal(m.logits(), got)
+        b.close()
+        m.close()
