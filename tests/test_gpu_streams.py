@@ -201,3 +201,91 @@ def test_a_model_refuses_the_graphs_that_cannot_be():
         assert np.array_equal(m.logits(), got)
         b.close()
         m.close()
+
+
+def test_a_captured_step_of_short_sequences(ex):
+    """A whole decode step without a workspace (append, attention of up to 256 positions, sampling of a small vocabulary) replayed with
+    lengths and tokens that the device moves on: each replay equals the eager calls of another executor."""
+    rng = np.random.default_rng(9)
+    n_seq, n_kv, n_heads, hd, vocab = 3, 2, 4, 64, 4 * 64
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream), HipKernelExecutor(0, stream=stream.cuda_stream) as mine:
+        b, t = paged_case(rng, [200, 17, 90], [1, 1, 1], n_kv, n_heads, hd)
+        other = {k: x.clone() for k, x in t.items()}
+        kv = [torch.randn(n_seq, n_kv * hd, device="cuda") for _ in range(2)]
+        u = torch.rand(n_seq, dtype=torch.float64, device="cuda")
+        start = t["kv_len"].clone() - 8
+        outs = []
+
+        def calls(e, t):
+            pool = e.wrap_paged_kv(borrowed(e, t["k"]), borrowed(e, t["v"]), b.n_pages, 16, n_kv, hd)
+            seqs = e.paged_seqs(borrowed(e, t["table"]), borrowed(e, t["kv_len"]), n_seq, b.max_blocks, None, 208)
+            out, token = torch.zeros_like(t["q"]), torch.zeros(n_seq, dtype=torch.int32, device="cuda")
+            bk, bv, bu, bq, bout, btok = (borrowed(e, x) for x in (*kv, u, t["q"], out, token))
+
+            def step():
+                e.paged_append_dev(pool, seqs, bk, bv, n_seq, q=bq, q_out=bout, n_heads=n_heads)
+                e.paged_attn_decode_dev(pool, seqs, bout, n_heads, bout)
+                e.sample_dev(bout, n_seq, vocab, bu, btok)
+
+            return step, out, token
+
+        graph_step, out, token = calls(mine, t)
+        eager_step, out2, token2 = calls(ex, other)
+        graph = torch.cuda.CUDAGraph()
+        graph_step()                                                       # both once before the capture: it stores keys, too
+        stream.synchronize()
+        eager_step()
+        ex.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            graph_step()
+        for x in (t, other):
+            x["kv_len"].copy_(start)
+        for i in range(5):
+            for x in (*kv, t["q"]):
+                x.normal_()
+            other["q"].copy_(t["q"])
+            u.uniform_()
+            for x in (t, other):
+                x["kv_len"] += 1
+            graph.replay()
+            stream.synchronize()                                           # ex has a stream of its own: the host waits for both
+            eager_step()
+            ex.synchronize()
+            outs.append((out.clone(), token.clone()))
+            assert torch.equal(out, out2) and torch.equal(token, token2) and torch.equal(t["k"], other["k"])
+        assert not torch.equal(outs[0][0], outs[1][0])
+
+
+def test_two_threads_on_one_executor(ex):
+    """Split decode steps of two batches from two host threads: the calls take turns on the context and its workspace."""
+    import threading
+    rng = np.random.default_rng(10)
+    work, errors = [], []
+    for lens in ([2500, 3], [40, 900, 1700]):
+        b = ref.Batch(rng, lens, 16, 2, 64)
+        pool = ex.paged_kv(b.n_pages, 16, 2, 64)
+        k, v = pool.pages()
+        k.upload(b.k.view(np.uint16)), v.upload(b.v.view(np.uint16))
+        seqs = ex.paged_seqs(ex.to_device(b.table), ex.to_device(b.kv_len), b.n_seq, b.max_blocks, None, max(lens))
+        q = rng.standard_normal((b.n_seq, 4 * 64)).astype(np.float32)
+        work.append((pool, seqs, ex.to_device(q), [ex.buffer(q.nbytes) for _ in range(40)], ex.buffer(q.nbytes)))
+    for pool, seqs, q, outs, first in work:
+        ex.paged_attn_decode_dev(pool, seqs, q, 4, first)
+
+    def loop(pool, seqs, q, outs, first):
+        try:
+            for o in outs:
+                ex.paged_attn_decode_dev(pool, seqs, q, 4, o)
+        except Exception as e:      # noqa: BLE001  (reported by the main thread)
+            errors.append(e)
+
+    threads = [threading.Thread(target=loop, args=w) for w in work]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not errors
+    for _, _, _, outs, first in work:
+        want = first.download(np.float32)
+        assert np.isfinite(want).all() and all(np.array_equal(o.download(np.float32), want) for o in outs)
